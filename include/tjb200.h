@@ -15,7 +15,8 @@
  *     graph.
  *   - Return 0 (TJB_OK) on success, otherwise a tjb_status code; no exception
  *     crosses the ABI.  tjb_status_string() names a code.
- *   - Dtype codes: TJB_F32 = 0, TJB_F16 = 1, TJB_BF16 = 2.
+ *   - Dtype codes: TJB_F32 = 0, TJB_F16 = 1, TJB_BF16 = 2; TJB_E4M3 = 3 only
+ *     where an entry point names it (block-scaled 8-bit operands).
  *   - Row-major matrices; leading dimensions are in elements.  Tensor-memory
  *     (TMA) operands need 16-byte aligned base pointers and row pitches.
  *   - Device-side waits are bounded.  A wait that runs out records
@@ -49,7 +50,7 @@ enum tjb_status {
   TJB_ERR_NON_PREFIX_MASK = 9    /* reported by tjb_mask_lengths' flag word */
 };
 
-enum tjb_dtype { TJB_F32 = 0, TJB_F16 = 1, TJB_BF16 = 2 };
+enum tjb_dtype { TJB_F32 = 0, TJB_F16 = 1, TJB_BF16 = 2, TJB_E4M3 = 3 };
 
 /* Library version (major*10000 + minor*100 + patch). */
 int tjb_version(void);
@@ -386,6 +387,67 @@ int tjb_forward_small(const tjb_small_layer* layers, int L, const float* lnf_w,
                       const float* lnf_b, float lnf_eps, const float* x, float* out,
                       const uint8_t* valid, int B, int S, int d, int H, int F, int causal,
                       int dtype, void* workspace, size_t workspace_bytes, tjb_stream_t stream);
+
+/*
+ * Block-scaled e4m3.  A block of values y (1 row x 128 columns for
+ * activations, 128 x 128 for weights; shorter at the edges) is held as
+ * q = e4m3(y / s), round to nearest even and saturating, with the fp32 scale
+ * s = max(amax|y| / 448, 2^-126).  A NaN or an infinity in a block makes its
+ * scale NaN or infinite and every value the block stands for NaN.
+ *
+ * tjb_quantize_blocks: x [rows, K] (in_dtype f32, f16 or bf16; rows ldx
+ * elements apart) -> q [rows, K] e4m3 and scales [rows, ceil(K/128)], both
+ * contiguous.  K % 16 == 0, ldx % 4 == 0; x aligned to four elements, q to
+ * 16 bytes.  m_tiles (nullable) as in tjb_row_tiles: rows of unlisted tiles
+ * are neither read nor written.
+ * tjb_quantize_weight_blocks: w [N, K] (rows ldw elements apart) ->
+ * q [N, K] and scales [ceil(N/128), ceil(K/128)]; same rules.
+ * No counterpart in the reference (fp16 operands only).
+ */
+int tjb_quantize_blocks(const void* x, int64_t ldx, int in_dtype, void* q, float* scales,
+                        int64_t rows, int K, const int32_t* m_tiles, tjb_stream_t stream);
+int tjb_quantize_weight_blocks(const void* w, int64_t ldw, int in_dtype, void* q, float* scales,
+                               int64_t N, int K, tjb_stream_t stream);
+
+/*
+ * Residual addition and root-mean-square norm over rows of length d:
+ *   x       = res + delta              (fp32; delta may be NULL: x = res)
+ *   res_out = x                        (rounded to res_dtype; skipped when NULL)
+ *   out     = x * rsqrt(mean(x^2) + eps) * w     in out_dtype
+ * The norm reads the unrounded sum.  res, res_out: res_dtype; delta:
+ * delta_dtype (each f32, f16 or bf16); w: fp32 [d]; out: f32, f16, bf16, or
+ * TJB_E4M3 with out_scales [rows, ceil(d/128)] (see tjb_quantize_blocks;
+ * ignored otherwise).  All contiguous; res_out may alias res.  d <= 16384,
+ * d % 4 == 0 (e4m3: d % 16 == 0).  row_mask (nullable): rows with 0 get a
+ * zero output row; m_tiles (nullable) as in tjb_row_tiles.
+ * The 8-bit-capable RMS sibling of fused_add_layernorm
+ * (tjkernels/kernels/__init__.py:48-70); no counterpart in the reference.
+ */
+int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out, void* out,
+                    float* out_scales, const float* w, int64_t rows, int d, float eps,
+                    int res_dtype, int delta_dtype, int out_dtype, const uint8_t* row_mask,
+                    const int32_t* m_tiles, tjb_stream_t stream);
+
+/*
+ * Product of block-scaled e4m3 matrices (see tjb_quantize_blocks):
+ *   C[m, n] = act( sum_kb sa[m, kb] sw[n/128, kb] sum_{k in kb} A[m, k] W[n, k]
+ *                  + bias[n] )
+ * A [M, K] e4m3 (rows lda bytes apart) with scales sa[m, kb] at
+ * a_scales[m * a_scales_row + kb * a_scales_blk]; W [N, K] e4m3 (rows ldw
+ * bytes apart) with w_scales contiguous [ceil(N/128), ceil(K/128)]; bias fp32
+ * [N] or NULL; act: 0 = none, 1 = exact erf GELU.  C (rows ldc elements
+ * apart): f32, f16, bf16, or TJB_E4M3 with c_scales contiguous
+ * [M, ceil(N/128)].  fp32 accumulation; a call's result depends on nothing
+ * but its operands (no atomics, no workspace).  K % 16 == 0, N % 8 == 0
+ * (e4m3 output: N % 16 == 0), lda and ldw multiples of 16, ldc of 8 (e4m3:
+ * 16); 16-byte aligned A, W, C and bias.  m_tiles (nullable) as in
+ * tjb_row_tiles.
+ * The 8-bit sibling of tjb_gemm_bias; no counterpart in the reference.
+ */
+int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scales_row,
+                 int64_t a_scales_blk, const void* W, const float* w_scales, const float* bias,
+                 void* C, float* c_scales, int M, int N, int K, int lda, int ldw, int ldc,
+                 int out_dtype, int act, const int32_t* m_tiles, tjb_stream_t stream);
 
 /*
  * Self-test of the bounded device-side wait: one thread spins on *flag

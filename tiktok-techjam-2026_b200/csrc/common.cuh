@@ -650,7 +650,7 @@ int make_tmap_16bit(CUtensorMap* map, int rank, const void* base, const uint64_t
                     const uint64_t* strides_bytes, const uint32_t* box, bool bf16);
 
 // 2-D tiled tensor map with 128-byte swizzle over a row-major matrix of
-// `dtype` (TJB_F32 / TJB_F16 / TJB_BF16): `cols` x `rows`, rows `ld_bytes`
+// `dtype` (TJB_F32 / TJB_F16 / TJB_BF16 / TJB_E4M3): `cols` x `rows`, rows `ld_bytes`
 // apart, box of box_cols x box_rows (box_cols * element size = 128 bytes).
 int make_tmap_2d(CUtensorMap* map, int dtype, const void* base, uint64_t cols, uint64_t rows,
                  uint64_t ld_bytes, uint32_t box_cols, uint32_t box_rows);

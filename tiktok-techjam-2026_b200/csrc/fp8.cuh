@@ -1,0 +1,122 @@
+// fp8.cuh -- block-scaled e4m3: the quantisation rule, packing, and the
+// 8-bit form of the tensor-core instruction, shared by rmsnorm.cu,
+// quantize.cu and gemm_fp8.cu.
+//
+// A block of values y (1 x 128 along a row for activations, 128 x 128 for
+// weights) is held as q = e4m3(y / s), round to nearest even, with the fp32
+// scale s = max(amax|y| / 448, 2^-126); 448 is the largest e4m3 value.  The
+// lower limit keeps y / s finite for a block of zeros or subnormals.  A NaN or
+// an infinity makes s NaN or infinite, and so every value the block stands
+// for NaN (finite / inf = 0, and 0 * inf is NaN).
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace tjb {
+
+constexpr int kQBlock = 128;      // columns (and weight rows) per scale
+constexpr int kLiveTileRows = 128;  // rows per entry of a live-tile list
+
+// |v| as an integer: ordered like the magnitude, with NaN above infinity, so
+// an integer maximum propagates both.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t abs_bits4(float4 v) {
+  return max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
+}
+
+// Scale of a block whose largest magnitude has these bits.
+__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
+  const float s = __uint_as_float(amax_bits) / 448.f;
+  return s < 1.17549435e-38f ? 1.17549435e-38f : s;  // a NaN stays a NaN
+}
+
+// Four e4m3 bytes of v / s, the first in the lowest byte.  True division:
+// multiplying by 1 / s moves about one value in 10^6 across a rounding border.
+__device__ __forceinline__ uint32_t quantize4(float4 v, float s) {
+  const __nv_fp8x2_storage_t lo =
+      __nv_cvt_float2_to_fp8x2(make_float2(v.x / s, v.y / s), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi =
+      __nv_cvt_float2_to_fp8x2(make_float2(v.z / s, v.w / s), __NV_SATFINITE, __NV_E4M3);
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+
+// Four consecutive elements of a row: raw as loaded (16 or 8 bytes), widened
+// to fp32 when they are used, so that a load in flight is not waited for.
+template <bool k16>
+struct Raw4;
+template <>
+struct Raw4<false> {
+  float4 v;
+};
+template <>
+struct Raw4<true> {
+  uint2 v;
+};
+
+template <bool k16>
+__device__ __forceinline__ Raw4<k16> load_raw4(const void* p, int64_t idx) {
+  Raw4<k16> r;
+  if constexpr (k16)
+    r.v = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + idx));
+  else
+    r.v = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(p) + idx));
+  return r;
+}
+
+template <bool k16>
+__device__ __forceinline__ float4 widen4(const Raw4<k16>& r, bool bf16) {
+  if constexpr (!k16) {
+    return r.v;
+  } else {
+    float2 a, b;
+    if (bf16) {
+      a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.v.x));
+      b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.v.y));
+    } else {
+      a = __half22float2(*reinterpret_cast<const __half2*>(&r.v.x));
+      b = __half22float2(*reinterpret_cast<const __half2*>(&r.v.y));
+    }
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+
+// Four consecutive fp32 values rounded once to `dtype` (f32, f16, bf16).
+__device__ __forceinline__ void store4(void* out, int dtype, int64_t idx, float4 y) {
+  if (dtype == TJB_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + idx) = y;
+    return;
+  }
+  uint2 raw;
+  if (dtype == TJB_BF16) {
+    raw.x = Pack2<__nv_bfloat16>::pack(y.x, y.y);
+    raw.y = Pack2<__nv_bfloat16>::pack(y.z, y.w);
+  } else {
+    raw.x = Pack2<__half>::pack(y.x, y.y);
+    raw.y = Pack2<__half>::pack(y.z, y.w);
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + idx) = raw;
+}
+
+// Instruction descriptor of kind::f8f6f4 with e4m3 operands (format 0), fp32
+// accumulation, both K-major; the fields sit as in idesc_f16.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// D[tmem] (+)= A[smem] * B[smem] over K = 32 e4m3 columns; warp-collective
+// like umma_ss_w.
+__device__ __forceinline__ void umma_e4m3_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+}  // namespace tjb

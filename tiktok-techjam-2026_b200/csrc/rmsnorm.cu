@@ -1,0 +1,166 @@
+// rmsnorm.cu -- residual addition + root-mean-square norm (HBM-bound).
+//
+//   x = res + delta (fp32),  out = x * rsqrt(mean(x^2) + eps) * w
+// The new residual is x rounded once to the residual's type; the norm reads
+// the unrounded fp32 sum.  The output is f32 / f16 / bf16, or e4m3 with one
+// scale for each row and 128 columns.
+//
+// One row is owned by TPR threads, chunk i of thread t covering columns
+// 4 (i TPR + t) .. +3: the 32 lanes of a warp hold 128 consecutive, aligned
+// columns of a chunk, which is exactly one scale block, so its amax is one
+// warp-wide integer maximum of values already in registers.
+#include "fp8.cuh"
+
+namespace tjb {
+namespace {
+
+constexpr int kRmsChunks = 8;  // row chunks a thread holds: d <= 32 TPR
+
+// Sum over the TPR threads of a row; every thread of the block calls it.
+template <int TPR>
+__device__ __forceinline__ float rms_row_sum(float v, float* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (TPR > 32) {
+    constexpr int kWarps = TPR / 32;
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) scratch[warp] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) v += scratch[warp / kWarps * kWarps + i];
+  }
+  return v;
+}
+
+// kDelta: 0 none, 1 fp32, 2 sixteen bits.
+template <int TPR, int BLOCK, bool kRes16, int kDelta>
+__global__ void __launch_bounds__(BLOCK)
+    add_rmsnorm_kernel(const void* res, const void* delta, void* res_out, void* out,
+                       float* __restrict__ out_scales, const float* __restrict__ w, int rows,
+                       int d, float eps, int res_dtype, int delta_dtype, int out_dtype,
+                       const uint8_t* __restrict__ row_mask,
+                       const int32_t* __restrict__ m_tiles) {
+  constexpr int kRowsPerBlock = BLOCK / TPR;
+  __shared__ float scratch[BLOCK / 32];
+  const int t = threadIdx.x % TPR;
+  griddep_wait();
+  griddep_launch_dependents();
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + threadIdx.x / TPR;
+  if (m_tiles != nullptr) {
+    // Rows are numbered over the listed 128-row tiles (uniform per block).
+    const int64_t li = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock / kLiveTileRows;
+    if (li >= __ldg(m_tiles)) return;
+    row = static_cast<int64_t>(__ldg(m_tiles + 1 + li)) * kLiveTileRows + row % kLiveTileRows;
+  }
+  const bool active = row < rows;
+  const int64_t base = row * d;
+  Raw4<kRes16> rr[kRmsChunks];
+  Raw4<kDelta == 2> rd[kDelta == 0 ? 1 : kRmsChunks];
+#pragma unroll
+  for (int i = 0; i < kRmsChunks; ++i) {
+    const int col = (i * TPR + t) * 4;
+    if (active && col < d) {
+      rr[i] = load_raw4<kRes16>(res, base + col);
+      if constexpr (kDelta != 0) rd[i] = load_raw4<kDelta == 2>(delta, base + col);
+    }
+  }
+  float4 v[kRmsChunks];
+  float sq = 0.f;
+#pragma unroll
+  for (int i = 0; i < kRmsChunks; ++i) {
+    const int col = (i * TPR + t) * 4;
+    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (active && col < d) {
+      v[i] = widen4<kRes16>(rr[i], res_dtype == TJB_BF16);
+      if constexpr (kDelta != 0) {
+        const float4 dl = widen4<kDelta == 2>(rd[i], delta_dtype == TJB_BF16);
+        v[i].x += dl.x;
+        v[i].y += dl.y;
+        v[i].z += dl.z;
+        v[i].w += dl.w;
+      }
+      sq += (v[i].x * v[i].x + v[i].y * v[i].y) + (v[i].z * v[i].z + v[i].w * v[i].w);
+    }
+  }
+  const float mean = rms_row_sum<TPR>(sq, scratch) / static_cast<float>(d);
+  const float rstd = __frsqrt_rn(mean + eps);
+  if (!active) return;  // uniform over each warp
+  const bool keep = row_mask == nullptr || __ldg(row_mask + row) != 0;
+  const int kb_count = (d + kQBlock - 1) / kQBlock;
+#pragma unroll
+  for (int i = 0; i < kRmsChunks; ++i) {
+    const int col = (i * TPR + t) * 4;
+    const int kb = (i * TPR + t) >> 5;  // scale block of this warp's chunk
+    if (kb >= kb_count) break;          // warp-uniform
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col < d) {
+      if (res_out != nullptr) store4(res_out, res_dtype, base + col, v[i]);
+      if (keep) {
+        const float4 ww = __ldg(reinterpret_cast<const float4*>(w + col));
+        y.x = v[i].x * rstd * ww.x;
+        y.y = v[i].y * rstd * ww.y;
+        y.z = v[i].z * rstd * ww.z;
+        y.w = v[i].w * rstd * ww.w;
+      }
+    }
+    if (out_dtype == TJB_E4M3) {
+      const float s = block_scale(__reduce_max_sync(0xffffffffu, abs_bits4(y)));
+      if (col < d)
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + base + col) = quantize4(y, s);
+      if ((t & 31) == 0) out_scales[row * kb_count + kb] = s;
+    } else if (col < d) {
+      store4(out, out_dtype, base + col, y);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace tjb
+
+extern "C" int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out, void* out,
+                               float* out_scales, const float* w, int64_t rows, int d, float eps,
+                               int res_dtype, int delta_dtype, int out_dtype,
+                               const uint8_t* row_mask, const int32_t* m_tiles,
+                               tjb_stream_t stream) {
+  using namespace tjb;
+  if (!res || !out || !w || rows < 0 || d <= 0) return TJB_ERR_INVALID_ARGUMENT;
+  if (res_dtype < TJB_F32 || res_dtype > TJB_BF16 || delta_dtype < TJB_F32 ||
+      delta_dtype > TJB_BF16 || out_dtype < TJB_F32 || out_dtype > TJB_E4M3)
+    return TJB_ERR_UNSUPPORTED_DTYPE;
+  const bool q = out_dtype == TJB_E4M3;
+  if (q && !out_scales) return TJB_ERR_INVALID_ARGUMENT;
+  if (d % (q ? 16 : 4) != 0 || d > 16384 || rows > 2147483647 - kLiveTileRows)
+    return TJB_ERR_BAD_SHAPE;
+  // Vectors of four elements.
+  auto misaligned = [](const void* p, int dtype) {
+    return (reinterpret_cast<uintptr_t>(p) & (dtype == TJB_F32 ? 15u : 7u)) != 0;
+  };
+  if (misaligned(res, res_dtype) || (delta && misaligned(delta, delta_dtype)) ||
+      (res_out && misaligned(res_out, res_dtype)) || !aligned16(w) || misaligned(out, out_dtype) ||
+      (q && (!aligned16(out) || (reinterpret_cast<uintptr_t>(out_scales) & 3u) != 0)))
+    return TJB_ERR_BAD_ALIGNMENT;
+  if (!device_ok()) return TJB_ERR_NO_DEVICE;
+  if (rows == 0) return TJB_OK;
+  const int64_t n = m_tiles ? (rows + kLiveTileRows - 1) / kLiveTileRows * kLiveTileRows : rows;
+  auto go = [&](auto kern, int block, int per_block) {
+    return launch_kernel(kern, dim3(static_cast<unsigned>((n + per_block - 1) / per_block)),
+                         dim3(block), 0, reinterpret_cast<cudaStream_t>(stream), res, delta,
+                         res_out, out, out_scales, w, static_cast<int>(rows), d, eps, res_dtype,
+                         delta_dtype, out_dtype, row_mask, m_tiles);
+  };
+  auto pick = [&](auto res16, auto kdelta) {
+    constexpr bool R = decltype(res16)::value;
+    constexpr int D = decltype(kdelta)::value;
+    if (d <= 32 * 32) return go(add_rmsnorm_kernel<32, 256, R, D>, 256, 8);
+    if (d <= 32 * 128) return go(add_rmsnorm_kernel<128, 256, R, D>, 256, 2);
+    if (d <= 32 * 256) return go(add_rmsnorm_kernel<256, 256, R, D>, 256, 1);
+    return go(add_rmsnorm_kernel<512, 512, R, D>, 512, 1);
+  };
+  auto with_delta = [&](auto res16) {
+    if (!delta) return pick(res16, std::integral_constant<int, 0>{});
+    if (delta_dtype == TJB_F32) return pick(res16, std::integral_constant<int, 1>{});
+    return pick(res16, std::integral_constant<int, 2>{});
+  };
+  return res_dtype == TJB_F32 ? with_delta(std::false_type{}) : with_delta(std::true_type{});
+}

@@ -94,6 +94,7 @@ int make_tmap_2d(CUtensorMap* map, int dtype, const void* base, uint64_t cols, u
   if (g_encode == nullptr) return TJB_ERR_TENSOR_MAP;
   const CUtensorMapDataType dt = dtype == TJB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : dtype == TJB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : dtype == TJB_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   cuuint64_t gdim[2] = {cols, rows};
   cuuint64_t gstride[1] = {ld_bytes};

@@ -8,3 +8,6 @@
 #include "ffn.cu"
 #include "ffn_fused.cu"
 #include "forward_small.cu"
+#include "quantize.cu"
+#include "rmsnorm.cu"
+#include "gemm_fp8.cu"

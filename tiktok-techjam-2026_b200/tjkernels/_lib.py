@@ -14,7 +14,7 @@ from pathlib import Path
 # The in-tree build (tiktok-techjam-2026_b200/build.py writes it here).
 LIB_PATH = Path(__file__).resolve().with_name("libtjb200.so")
 
-TJB_F32, TJB_F16, TJB_BF16 = 0, 1, 2
+TJB_F32, TJB_F16, TJB_BF16, TJB_E4M3 = 0, 1, 2, 3
 
 _c_int, _c_i64, _c_f32, _p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -63,6 +63,12 @@ SIGNATURES = {
     "tjb_forward_small": (_c_int, [_p, _c_int, _p, _p, _c_f32, _p, _p, _p, _c_int, _c_int,
                                    _c_int, _c_int, _c_int, _c_int, _c_int, _p, ctypes.c_size_t,
                                    _p]),
+    "tjb_quantize_blocks": (_c_int, [_p, _c_i64, _c_int, _p, _p, _c_i64, _c_int, _p, _p]),
+    "tjb_quantize_weight_blocks": (_c_int, [_p, _c_i64, _c_int, _p, _p, _c_i64, _c_int, _p]),
+    "tjb_add_rmsnorm": (_c_int, [_p, _p, _p, _p, _p, _p, _c_i64, _c_int, _c_f32, _c_int, _c_int,
+                                 _c_int, _p, _p, _p]),
+    "tjb_gemm_fp8": (_c_int, [_p, _p, _c_i64, _c_i64, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int,
+                              _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p]),
 }
 
 

@@ -10,6 +10,9 @@ Same functions and argument meaning as the reference facade
 Differences by design: there is no Triton and no torch fallback.  Every call
 runs the CUDA library on the tensor's device and current stream; a CPU tensor,
 an unsupported shape or dtype raises instead of silently switching backend.
+Beside them stands the block-scaled 8-bit path: ``fused_add_rmsnorm``,
+``quantize_blocks``, ``quantize_weight_blocks`` and ``gemm_fp8``, for which the
+reference has no counterpart.
 Outputs are allocated here with ``torch.empty`` (the caching allocator, so the
 calls capture into CUDA graphs); the library itself never allocates.
 """
@@ -432,6 +435,222 @@ def forward_small(model: SmallModel, x: torch.Tensor, valid: Optional[torch.Tens
     return out
 
 
+# ------------------------------------------------- block-scaled 8-bit operators
+# A matrix held in e4m3 is a pair (q, scales): q float8_e4m3fn [R, K]; scales
+# fp32, one for each row and 128 columns (activations) or one for each
+# 128 x 128 block (weights).  The value held is q * its block's scale.
+
+SCALE_BLOCK = 128
+
+
+def _blocks(n: int) -> int:
+    return (n + SCALE_BLOCK - 1) // SCALE_BLOCK
+
+
+def _need_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+    """The CUDA device that every given tensor is on."""
+    _need_cuda(first, *others)
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}: one call runs on one device")
+    return device
+
+
+def _launch(what: str, device: torch.device, *args) -> None:
+    """Call C entry point ``what`` with ``args`` and the current stream of
+    ``device``, which need not be the current device."""
+    fn = getattr(_lib.lib(), what)
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _stream(device))
+    _lib.check(status, what)
+
+
+def _rows(t: torch.Tensor, unit: int) -> Tuple[torch.Tensor, int]:
+    """``t`` [R, C] as rows of consecutive elements that start at multiples of
+    ``unit`` elements (copied when they do not), and the row pitch."""
+    r, c = t.shape
+    pitch = t.stride(0) if r > 1 else -(-c // unit) * unit
+    if t.stride(1) != 1 or pitch < c or pitch % unit != 0 \
+            or t.data_ptr() % (unit * t.element_size()) != 0:
+        t = t.clone(memory_format=torch.contiguous_format)
+        pitch = c
+    return t, pitch
+
+
+def _check_tiles(m_tiles: Optional[torch.Tensor], rows: int) -> None:
+    if m_tiles is not None and (m_tiles.dtype != torch.int32 or not m_tiles.is_contiguous()
+                                or m_tiles.numel() < 1 + (rows + 127) // 128):
+        raise ValueError("m_tiles must be the int32 tile list of row_tiles for this row count")
+
+
+def quantize_blocks(x: torch.Tensor, m_tiles: Optional[torch.Tensor] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Activations ``x`` [R, K] (fp32, fp16 or bf16; rows at any pitch) to
+    block-scaled e4m3: ``(q [R, K], scales [R, ceil(K/128)])`` with
+    ``scale = max(amax / 448, 2**-126)`` over each row's 128 columns and
+    ``q = e4m3(x / scale)``.  K must be a multiple of 16.  A NaN or an infinity
+    makes its whole block NaN.  With ``m_tiles`` (from :func:`row_tiles`) only
+    the listed 128-row tiles are read and written."""
+    device = _need_device(x, m_tiles)
+    if x.dim() != 2:
+        raise ValueError("x must be [R, K]")
+    code = _code(x.dtype)
+    r, k = x.shape
+    _check_tiles(m_tiles, r)
+    q = torch.empty((r, k), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty((r, _blocks(k)), dtype=torch.float32, device=device)
+    if r:
+        x, ld = _rows(x, 4)
+        _launch("tjb_quantize_blocks", device, _ptr(x), ld, code, _ptr(q), _ptr(scales), r, k,
+                _ptr(m_tiles))
+    return q, scales
+
+
+def quantize_weight_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Weights ``w`` [N, K] (nn.Linear layout; fp32, fp16 or bf16) to
+    block-scaled e4m3: ``(q [N, K], scales [ceil(N/128), ceil(K/128)])``, one
+    scale for each 128 x 128 block, by the rule of :func:`quantize_blocks`."""
+    device = _need_device(w)
+    if w.dim() != 2:
+        raise ValueError("w must be [N, K]")
+    code = _code(w.dtype)
+    n, k = w.shape
+    q = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty((_blocks(n), _blocks(k)), dtype=torch.float32, device=device)
+    if n:
+        w, ld = _rows(w, 4)
+        _launch("tjb_quantize_weight_blocks", device, _ptr(w), ld, code, _ptr(q), _ptr(scales),
+                n, k)
+    return q, scales
+
+
+def fused_add_rmsnorm(
+    residual: torch.Tensor,
+    delta: Optional[torch.Tensor],
+    weight: torch.Tensor,
+    eps: float,
+    out_dtype: Optional[torch.dtype] = None,
+    write_residual: bool = True,
+    row_mask: Optional[torch.Tensor] = None,
+    residual_out: Optional[torch.Tensor] = None,
+    m_tiles: Optional[torch.Tensor] = None,
+):
+    """``x = residual + delta``; return ``(x, x * rsqrt(mean(x^2) + eps) * weight)``.
+
+    ``residual`` and ``delta`` (or None) are ``[rows, d]`` in fp32, fp16 or
+    bf16, each its own; ``weight`` fp32 ``[d]``.  The sum is fp32: the norm
+    reads it as it is, the returned residual is rounded once to its type.
+    With ``out_dtype=torch.float8_e4m3fn`` the second result is the pair
+    ``(q, scales)`` of :func:`quantize_blocks`, computed from the unrounded
+    norm (d a multiple of 16; otherwise of 4; at most 16384).
+    ``write_residual``, ``residual_out`` (may be ``residual``), ``row_mask``
+    and ``m_tiles`` as in :func:`fused_add_layernorm`."""
+    device = _need_device(residual, delta, weight, row_mask, residual_out, m_tiles)
+    if residual.dim() != 2 or not residual.is_contiguous():
+        raise ValueError("residual must be a contiguous [rows, d] tensor")
+    rows, d = residual.shape
+    if weight.dtype != torch.float32 or weight.shape != (d,) or not weight.is_contiguous():
+        raise ValueError("weight must be a contiguous fp32 [d] tensor")
+    code = _code(residual.dtype)
+    delta_code = _lib.TJB_F32
+    if delta is not None:
+        if delta.shape != residual.shape:
+            raise ValueError("delta must have the shape of residual")
+        delta_code = _code(delta.dtype)
+        if not delta.is_contiguous():
+            delta = delta.contiguous()
+    if row_mask is not None:
+        if row_mask.dtype == torch.bool:
+            row_mask = row_mask.view(torch.uint8)
+        if row_mask.dtype != torch.uint8 or row_mask.numel() != rows \
+                or not row_mask.is_contiguous():
+            raise ValueError("row_mask must be a contiguous uint8 or bool mask of the rows")
+    _check_tiles(m_tiles, rows)
+    out_dtype = out_dtype or residual.dtype
+    scales = None
+    if out_dtype == torch.float8_e4m3fn:
+        out_code = _lib.TJB_E4M3
+        scales = torch.empty((rows, _blocks(d)), dtype=torch.float32, device=device)
+    else:
+        out_code = _code(out_dtype)
+    out = torch.empty((rows, d), dtype=out_dtype, device=device)
+    res_out = None
+    if write_residual and delta is not None:
+        if residual_out is None:
+            res_out = torch.empty_like(residual)
+        elif residual_out.shape != residual.shape or residual_out.dtype != residual.dtype \
+                or not residual_out.is_contiguous():
+            raise ValueError("residual_out must be contiguous, of residual's shape and dtype")
+        else:
+            res_out = residual_out
+    if rows:
+        _launch("tjb_add_rmsnorm", device, _ptr(residual), _ptr(delta), _ptr(res_out), _ptr(out),
+                _ptr(scales), _ptr(weight), rows, d, float(eps), code, delta_code, out_code,
+                _ptr(row_mask), _ptr(m_tiles))
+    return (res_out if res_out is not None else residual), \
+        (out if scales is None else (out, scales))
+
+
+def rmsnorm(x, weight, eps, out_dtype=None):
+    """Plain root-mean-square norm over the last dim, emitting ``out_dtype``
+    (for e4m3 the pair ``(q, scales)``)."""
+    return fused_add_rmsnorm(x, None, weight, eps, out_dtype=out_dtype, write_residual=False)[1]
+
+
+def gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+             bias: Optional[torch.Tensor] = None, act: int = ACT_NONE,
+             out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
+             m_tiles: Optional[torch.Tensor] = None):
+    """``act(A @ W.T + bias)`` of block-scaled e4m3 operands: ``a`` [M, K] with
+    ``a_scales`` [M, ceil(K/128)] (any strides), ``w`` [N, K] with contiguous
+    ``w_scales`` [ceil(N/128), ceil(K/128)]; bias fp32 [N].  Each 128-column
+    block's product is scaled and summed in fp32.  ``out_dtype`` fp32, fp16,
+    bf16, or float8_e4m3fn, which returns ``(q, scales)`` as
+    :func:`quantize_blocks` of the fp32 result would.  K must be a multiple of
+    16, N of 8 (e4m3 output: 16).  ``out``: a [M, N] tensor of ``out_dtype`` to
+    write (rows at any 16-byte pitch).  With ``m_tiles`` only the listed
+    128-row tiles are computed."""
+    device = _need_device(a, a_scales, w, w_scales, bias, out, m_tiles)
+    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
+        raise ValueError("a must be [M, K] and w [N, K]")
+    m, k = a.shape
+    n = w.shape[0]
+    if a.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn:
+        raise TypeError("a and w must be float8_e4m3fn")
+    if a_scales.dtype != torch.float32 or w_scales.dtype != torch.float32:
+        raise TypeError("scales are fp32")
+    if a_scales.shape != (m, _blocks(k)) or w_scales.shape != (_blocks(n), _blocks(k)):
+        raise ValueError("scales must be [M, ceil(K/128)] and [ceil(N/128), ceil(K/128)]")
+    if not w_scales.is_contiguous():
+        w_scales = w_scales.contiguous()
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,)
+                             or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous fp32 [N] tensor")
+    _check_tiles(m_tiles, m)
+    scales = None
+    if out_dtype == torch.float8_e4m3fn:
+        out_code, unit = _lib.TJB_E4M3, 16
+        scales = torch.empty((m, _blocks(n)), dtype=torch.float32, device=device)
+    else:
+        out_code, unit = _code(out_dtype), 8
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=device)
+    elif out.shape != (m, n) or out.dtype != out_dtype or (m and n > 1 and out.stride(1) != 1):
+        raise ValueError("out must be an [M, N] tensor of out_dtype with consecutive columns")
+    if m:
+        a, lda = _rows(a, 16)
+        w, ldw = _rows(w, 16)
+        ldc = out.stride(0) if m > 1 else -(-n // unit) * unit
+        _launch("tjb_gemm_fp8", device, _ptr(a), _ptr(a_scales), a_scales.stride(0),
+                a_scales.stride(1), _ptr(w), _ptr(w_scales), _ptr(bias), _ptr(out), _ptr(scales),
+                m, n, k, lda, ldw, ldc, out_code, act, _ptr(m_tiles))
+    return out if scales is None else (out, scales)
+
+
 __all__ = [
     "ACT_NONE", "ACT_GELU", "fused_add_layernorm", "layernorm", "gemm_bias", "gemm_workspace",
     "gemm_add_layernorm_workspace", "gemm_add_layernorm_workspace_bytes",
@@ -442,4 +661,6 @@ __all__ = [
     "device_status",
     "device_status_async",
     "forward_small", "forward_small_supports", "forward_small_workspace", "SmallModel",
+    "SCALE_BLOCK", "quantize_blocks", "quantize_weight_blocks", "fused_add_rmsnorm", "rmsnorm",
+    "gemm_fp8",
 ]
