@@ -41,6 +41,7 @@ struct GemmF8Args {
   int M, N, K, ldc;
   int out_dtype, act;
   int splits;  // CTAs per cluster (a power of two)
+  bool wide_stores;  // C and its rows start on 32-byte boundaries
 };
 
 template <int BT>
@@ -401,6 +402,520 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
                                static_cast<unsigned>(args.splits), tmW, tmX, args);
 }
 
+// ------------------------------------------------------------------------
+// Many tokens: 128 x 256 tiles of C per CTA (with CTAS = 2 a CTA pair shares
+// the MMAs of a 256 x 256 tile, CTA r holding token rows 128 r .. of it and
+// 128 of its 256 weight rows).  Here the tokens are the MMA's rows: a thread
+// owns one token and 128 consecutive output columns, which is one weight
+// block (one scale product per k-block) and one output block (its 8-bit scale
+// needs no exchange).  Persistent, 384 threads:
+//   warp 0        TMA producer
+//   warp 1        MMA issuer (leader CTA): per k-block four K = 32 MMAs into
+//                 one of two 256-column TMEM accumulators
+//   warps 2, 3    products sa[m, kb] sw[n / 128, kb] of the tile's rows, eight
+//                 k-blocks at a time, a ring slot ahead of their use
+//   warps 4..11   two warp groups, 128 columns each: read P_kb from TMEM in
+//                 16-column pieces, the next in flight while one is added to
+//                 128 fp32 sums in registers; then GELU, rounding, and 32-byte
+//                 stores (a thread holds 128 consecutive values of a row)
+// Per k-block and SM the tensor core takes 512 clocks (128 x 256 x 128 at
+// 8192 products a clock), the multiply-adds 280 (packed pairs, two clocks a
+// warp).  What bounds it is the chain MMA -> barrier -> scaling -> barrier ->
+// MMA over the two accumulators: every barrier operation, load and spilled
+// register in the k-loop adds to it.  The scaling threads need the registers
+// that warps 0-3 give up (128 x 72 + 256 x 216 = 384 x 168 at launch).
+template <int CTAS>
+struct WideCfg {
+  static constexpr int kStages = CTAS == 2 ? 6 : 4;
+  static constexpr int kThreads = 384;
+  static constexpr int kBRows = 256 / CTAS;       // weight rows a CTA holds per stage
+  static constexpr uint32_t kABytes = 128 * kF8BK;
+  static constexpr uint32_t kBBytes = kBRows * kF8BK;
+  static constexpr uint32_t kTmemCols = 512;      // two 256-column accumulators
+  static constexpr int kChunk = 8;                // k-blocks of scale products per ring slot
+  static constexpr uint32_t kScaleBytes = 2 * kChunk * 256 * 4;
+  static constexpr uint32_t kSmemBytes =
+      1024 + kStages * (kABytes + kBBytes) + kScaleBytes + 256;
+};
+
+__device__ __forceinline__ void umma_e4m3_pair_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                                 uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive on an mbarrier of another CTA of the cluster to hand back tensor
+// memory that this thread has finished reading.  The reads are complete and
+// ordered by tcgen05.fence, and no other memory is handed over, so the arrive
+// needs no release at cluster scope (whose fence, once per k-block, made the
+// kernel wait 4x the MMA time: 8192 x 4096 x 4096 328 us).
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t remote_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
+}
+
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+// 32 consecutive bytes of a row of which `cols` elements (per16 to 16 bytes)
+// exist; one 32-byte store where the matrix allows it (a thread holds a row,
+// so narrower stores would write each 32-byte sector twice).
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&w)[8], int cols, int per16,
+                                        bool wide) {
+  if (wide && cols >= 2 * per16) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+    return;
+  }
+  uint4* p = static_cast<uint4*>(dst);
+  if (cols >= per16) p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (cols >= 2 * per16) p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+template <int CTAS>
+__device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                     uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CTAS == 2)
+    umma_e4m3_pair_w(d_tmem, adesc, bdesc, idesc, accumulate);
+  else
+    umma_e4m3_w(d_tmem, adesc, bdesc, idesc, accumulate);
+}
+
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CTAS == 2)
+    umma_commit_pair_w(bar, 0x3);
+  else
+    umma_commit_w(bar);
+}
+
+// sum[0..15] += s * p[0..15]
+__device__ __forceinline__ void add_scaledN(float* sum, const uint32_t* p, float s) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 2)
+    fma2v(sum[j], sum[j + 1], __uint_as_float(p[j]), __uint_as_float(p[j + 1]), s, s, sum[j],
+          sum[j + 1]);
+}
+
+template <int CTAS>
+__global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
+    gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmA,
+                         const __grid_constant__ CUtensorMap tmB,
+                         const GemmF8Args args) {
+  using Cfg = WideCfg<CTAS>;
+  constexpr bool kPair = CTAS == 2;
+  constexpr int kStages = Cfg::kStages, kChunk = Cfg::kChunk;
+  constexpr int BN = 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + kStages * Cfg::kABytes;
+  float* sScale = reinterpret_cast<float*>(sB + kStages * Cfg::kBBytes);  // [slot][k-block][half][row]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sScale + 2 * kChunk * 256);  // leader's are used
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;
+  uint64_t* tempty = tfull + 2;  // leader's are used
+  uint64_t* sfull = tempty + 2;
+  uint64_t* sempty = sfull + 2;
+  uint64_t* drain = sempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kPair ? cluster_ctarank() : 0u;  // 0: the leader, which issues the MMAs
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);   // the leader's expect-tx arrival + both CTAs' bytes
+      mbar_init(&empty[s], 1);  // one commit of the leader's MMAs to both CTAs
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 8 * CTAS);  // eight scaling warps of each CTA
+      mbar_init(&sfull[b], 2);  // warps 2 and 3
+      mbar_init(&sempty[b], 8);  // the scaling warps
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+  }
+  if (warp == 1) {
+    if constexpr (kPair) {
+      tmem_alloc_pair(tmem_slot, Cfg::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, Cfg::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  // Both CTAs' barriers are initialised and their tensor memory allocated
+  // before either signals the other.
+  if constexpr (kPair)
+    cluster_sync();
+  else
+    __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int num_m = args.m_tiles != nullptr ? __ldg(args.m_tiles) : (args.M + 127) / 128;
+  const int num_mp = (num_m + CTAS - 1) / CTAS;
+  const int num_n = (args.N + BN - 1) / BN;
+  const int num_k = (args.K + kF8BK - 1) / kF8BK;
+  const int num_tiles = num_mp * num_n;
+  const int first = static_cast<int>(blockIdx.x) / CTAS;
+  const int step = static_cast<int>(gridDim.x) / CTAS;
+  // This CTA's 128 token rows of pair tile t.  A pair whose second 128-row
+  // tile does not exist loads the first one's rows again (the MMA needs both
+  // halves) and its second CTA stores nothing.
+  auto coords = [&](int t, int& m_blk, int& n_blk) {
+    int mp;
+    tile_coords(t, num_mp, num_n, mp, n_blk);
+    int mt = CTAS * mp + static_cast<int>(rank);
+    const bool has = mt < num_m;
+    if (!has) mt = CTAS * mp;
+    m_blk = args.m_tiles != nullptr ? __ldg(args.m_tiles + 1 + mt) : mt;
+    return has;
+  };
+
+  if (warp < 4) {
+    regs_dec<72>();
+    if (warp == 0 && lane == 0) {
+      // ------------------------------------------------------------ producer
+      const uint32_t full_leader = kPair ? map_to_rank(smem_u32(full), 0) : 0u;
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, last_parity = 0;
+      bool ok = true;
+      for (int t = first; ok && t < num_tiles; t += step) {
+        int m_blk, n_blk;
+        coords(t, m_blk, n_blk);
+        for (int kb = 0; kb < num_k; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0)
+            mbar_arrive_expect_tx(&full[stage], CTAS * (Cfg::kABytes + Cfg::kBBytes));
+          uint8_t* a = sA + stage * Cfg::kABytes;
+          uint8_t* b = sB + stage * Cfg::kBBytes;
+          const int brow = n_blk * BN + static_cast<int>(rank) * Cfg::kBRows;
+          if constexpr (kPair) {
+            const uint32_t bar = full_leader + static_cast<uint32_t>(stage) * 8u;
+            tma_load_2d_pair(a, &tmA, bar, kb * kF8BK, m_blk * 128);
+            tma_load_2d_pair(b, &tmB, bar, kb * kF8BK, brow);
+          } else {
+            tma_load_2d(a, &tmA, &full[stage], kb * kF8BK, m_blk * 128);
+            tma_load_2d(b, &tmB, &full[stage], kb * kF8BK, brow);
+          }
+          issued |= 1u << stage;
+          last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // Every load this CTA issued has landed once the MMAs that read it
+      // have released its stage (the loads count on the leader's barrier).
+      for (int s = 0; s < kStages; ++s)
+        if ((issued >> s) & 1u) mbar_wait_drain(&empty[s], (last_parity >> s) & 1u);
+    } else if (warp == 1 && rank == 0) {
+      // ---------------------------------------------- MMA issuer (leader only)
+      constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, BN);
+      int stage = 0;
+      uint32_t phase = 0, it = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+      };
+      for (int t = first; ok && t < num_tiles; t += step) {
+        for (int kb = 0; kb < num_k; ++kb, ++it) {
+          const uint32_t acc = it & 1;
+          if (!wait(&full[stage], phase) || !wait(&tempty[acc], ((it >> 1) & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + stage * Cfg::kABytes);
+          const uint32_t b0 = smem_u32(sB + stage * Cfg::kBBytes);
+#pragma unroll
+          for (int k = 0; k < kF8BK / 32; ++k)
+            umma<CTAS>(tmem_base + acc * BN, sdesc_sw128(a0 + k * 32, 16, 1024),
+                       sdesc_sw128(b0 + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
+          commit<CTAS>(&tfull[acc]);
+          commit<CTAS>(&empty[stage]);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if constexpr (kPair)
+        umma_commit_pair_w(drain, 0x1);
+      else
+        umma_commit_w(drain);
+      mbar_wait_drain(drain, 0);
+    } else if (warp >= 2) {
+      // --------------------------------------------------------- scale products
+      // Warps 2 and 3 take 64 rows each, two per lane.
+      const int num_nb = (args.N + kQBlock - 1) / kQBlock;
+      const int r = (warp - 2) * 64 + lane;
+      // Row-major scales whose rows start on 16-byte boundaries: four at a time.
+      const bool vec = args.as_blk == 1 && args.as_row % 4 == 0 &&
+                       (reinterpret_cast<uintptr_t>(args.a_scales) & 15u) == 0;
+      uint32_t c = 0;
+      bool ok = true;
+      for (int t = first; ok && t < num_tiles; t += step) {
+        int m_blk, n_blk;
+        coords(t, m_blk, n_blk);
+        const int64_t row = static_cast<int64_t>(m_blk) * 128 + r;
+        // Rows past M and columns past N repeat an existing one: their sums
+        // are never stored.
+        const float* a0 = args.a_scales + min(row, static_cast<int64_t>(args.M - 1)) * args.as_row;
+        const float* a1 =
+            args.a_scales + min(row + 32, static_cast<int64_t>(args.M - 1)) * args.as_row;
+        const float* w0 = args.w_scales + static_cast<int64_t>(2 * n_blk) * num_k;
+        const float* w1 = 2 * n_blk + 1 < num_nb ? w0 + num_k : w0;
+        for (int kb0 = 0; ok && kb0 < num_k; kb0 += kChunk, ++c) {
+          float va[kChunk], vb[kChunk], s0[kChunk], s1[kChunk];
+          if (vec && kb0 + kChunk <= num_k) {
+#pragma unroll
+            for (int u = 0; u < kChunk; u += 4) {
+              *reinterpret_cast<float4*>(va + u) = __ldg(reinterpret_cast<const float4*>(a0 + kb0 + u));
+              *reinterpret_cast<float4*>(vb + u) = __ldg(reinterpret_cast<const float4*>(a1 + kb0 + u));
+            }
+#pragma unroll
+            for (int u = 0; u < kChunk; ++u) {
+              s0[u] = __ldg(w0 + kb0 + u);
+              s1[u] = __ldg(w1 + kb0 + u);
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < kChunk; ++u) {
+              const int kb = min(kb0 + u, num_k - 1);
+              va[u] = __ldg(a0 + kb * args.as_blk);
+              vb[u] = __ldg(a1 + kb * args.as_blk);
+              s0[u] = __ldg(w0 + kb);
+              s1[u] = __ldg(w1 + kb);
+            }
+          }
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&sempty[c & 1], ((c >> 1) & 1) ^ 1, abort_flag));
+          float* dst = sScale + (c & 1) * kChunk * 256 + r;
+#pragma unroll
+          for (int u = 0; u < kChunk; ++u) {
+            dst[u * 256] = va[u] * s0[u];
+            dst[u * 256 + 32] = vb[u] * s0[u];
+            dst[u * 256 + 128] = va[u] * s1[u];
+            dst[u * 256 + 160] = vb[u] * s1[u];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sfull[c & 1]);
+        }
+      }
+    }
+  } else {
+    regs_inc<216>();
+    // ------------------------------------------------- scaling and output
+    const int quad = warp & 3;         // TMEM lanes this warp may access
+    const int half = (warp - 4) >> 2;  // 128-column half of the tile
+    const int r = quad * 32 + lane;    // token row of the tile
+    const uint32_t tempty_leader = kPair ? map_to_rank(smem_u32(tempty), 0) : 0u;
+    const uint32_t taddr0 =
+        tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 128);
+    uint32_t it = 0, chunk = 0;  // k-blocks and scale chunks done, over all tiles
+    bool ok = true;
+    for (int t = first; ok && t < num_tiles; t += step) {
+      int m_blk, n_blk;
+      const bool has_rows = coords(t, m_blk, n_blk);
+      const int n0 = n_blk * BN + half * 128;
+      // The sums start from the bias; columns past N stay exactly zero (their
+      // weight rows load as zeros), as a ragged 8-bit block's scale needs.
+      float sum[128];
+#pragma unroll
+      for (int j = 0; j < 128; j += 4) {
+        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (args.bias != nullptr && n0 + j < args.N)
+          b = __ldg(reinterpret_cast<const float4*>(args.bias + n0 + j));
+        sum[j] = b.x;
+        sum[j + 1] = b.y;
+        sum[j + 2] = b.z;
+        sum[j + 3] = b.w;
+      }
+#pragma unroll 1
+      for (int kb = 0; kb < num_k; ++kb, ++it) {
+        const int u = kb & (kChunk - 1);
+        if (u == 0) ok = mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag) && ok;
+        const float s = sScale[((chunk & 1) * kChunk + u) * 256 + half * 128 + r];
+        const uint32_t acc = it & 1;
+        ok = mbar_wait(&tfull[acc], (it >> 1) & 1, abort_flag) && ok;
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t taddr = taddr0 + acc * BN;
+        uint32_t p[2][16];
+        tmem_ld16p(taddr, p[0]);
+        tmem_ld_wait_n<16>(p[0]);
+#pragma unroll
+        for (int c = 1; c < 128 / 16; ++c) {
+          tmem_ld16p(taddr + c * 16, p[c & 1]);
+          add_scaledN(sum + (c - 1) * 16, p[(c - 1) & 1], s);
+          tmem_ld_wait_n<16>(p[c & 1]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair)
+            mbar_arrive_remote(tempty_leader + acc * 8u);
+          else
+            mbar_arrive(&tempty[acc]);
+          if (u == kChunk - 1 || kb == num_k - 1) mbar_arrive(&sempty[chunk & 1]);
+        }
+        if (u == kChunk - 1 || kb == num_k - 1) ++chunk;
+        add_scaledN(sum + 128 - 16, p[1], s);
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (!has_rows || n0 >= args.N) continue;  // warp-uniform
+      if (args.act == 1) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) sum[j] = gelu_erf(sum[j]);
+      }
+      const int64_t row = static_cast<int64_t>(m_blk) * 128 + r;
+      if (row >= args.M) continue;
+      const int cols = min(args.N - n0, 128);
+      if (args.out_dtype == TJB_E4M3) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 128; ++j) top = max(top, abs_bits(sum[j]));
+        const float s = block_scale(top);
+        const float inv = __frcp_rn(s);
+        args.c_scales[row * ((args.N + kQBlock - 1) / kQBlock) + n0 / kQBlock] = s;
+        uint8_t* dst = static_cast<uint8_t*>(args.C) + row * args.ldc + n0;
+#pragma unroll
+        for (int j = 0; j < 128; j += 32) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = quantize4(&sum[j + 4 * i], s, inv);
+          store32(dst + j, w, cols - j, 16, args.wide_stores);
+        }
+      } else if (args.out_dtype == TJB_F32) {
+        float* dst = static_cast<float*>(args.C) + row * args.ldc + n0;
+#pragma unroll
+        for (int j = 0; j < 128; j += 8) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(sum[j + i]);
+          store32(dst + j, w, cols - j, 4, args.wide_stores);
+        }
+      } else {
+        uint16_t* dst = static_cast<uint16_t*>(args.C) + row * args.ldc + n0;
+#pragma unroll
+        for (int j = 0; j < 128; j += 16) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            w[i] = args.out_dtype == TJB_BF16
+                       ? Pack2<__nv_bfloat16>::pack(sum[j + 2 * i], sum[j + 2 * i + 1])
+                       : Pack2<__half>::pack(sum[j + 2 * i], sum[j + 2 * i + 1]);
+          store32(dst + j, w, cols - j, 8, args.wide_stores);
+        }
+      }
+    }
+  }
+
+  // Neither CTA releases its tensor memory (or exits) while the leader's
+  // MMAs or the peer's scaling warps may still touch the pair's resources.
+  __syncwarp();
+  tc_fence_before();
+  if constexpr (kPair)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    if constexpr (kPair)
+      tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    else
+      tmem_dealloc(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+int g_f8_wide[64][2];  // co-resident clusters per device and form (0: not yet known)
+
+template <int CTAS>
+int wide_resident(int& clusters) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return TJB_ERR_NO_DEVICE;
+  std::lock_guard<std::mutex> lock(g_f8_mu);
+  int& known = g_f8_wide[dev][CTAS - 1];
+  if (known == 0) {
+    if (const int fs = cuda_status(cudaFuncSetAttribute(
+            gemm_fp8_wide_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            static_cast<int>(WideCfg<CTAS>::kSmemBytes))))
+      return fs;
+    int n = num_sms();
+    if (CTAS == 2) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(2 * (num_sms() / 2));
+      cfg.blockDim = dim3(WideCfg<CTAS>::kThreads);
+      cfg.dynamicSmemBytes = WideCfg<CTAS>::kSmemBytes;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (const int qs = cuda_status(
+              cudaOccupancyMaxActiveClusters(&n, gemm_fp8_wide_kernel<CTAS>, &cfg)))
+        return qs;
+    }
+    known = n > 0 ? n : -1;
+  }
+  clusters = known;
+  return clusters > 0 ? TJB_OK : TJB_ERR_LAUNCH;
+}
+
+template <int CTAS>
+int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
+                cudaStream_t stream) {
+  using Cfg = WideCfg<CTAS>;
+  int clusters = 0;
+  if (const int st = wide_resident<CTAS>(clusters)) return st;
+  CUtensorMap tmA, tmB;
+  int st = make_tmap_2d(&tmA, TJB_E4M3, A, args.K, args.M, lda, kF8BK, 128);
+  if (st != TJB_OK) return st;
+  st = make_tmap_2d(&tmB, TJB_E4M3, W, args.K, args.N, ldw, kF8BK, Cfg::kBRows);
+  if (st != TJB_OK) return st;
+  const int64_t esz = args.out_dtype == TJB_F32 ? 4 : args.out_dtype == TJB_E4M3 ? 1 : 2;
+  args.wide_stores = ((reinterpret_cast<uintptr_t>(args.C) | (args.ldc * esz)) & 31) == 0;
+  const int64_t m_tiles = (static_cast<int64_t>(args.M) + 127) / 128;
+  const int64_t tiles = (m_tiles + CTAS - 1) / CTAS * ((args.N + 255) / 256);
+  if (tiles > 2147483647) return TJB_ERR_BAD_SHAPE;
+  const int n = tiles < clusters ? static_cast<int>(tiles) : clusters;
+  return launch_kernel_cluster(gemm_fp8_wide_kernel<CTAS>, dim3(CTAS * n), dim3(Cfg::kThreads),
+                               Cfg::kSmemBytes, stream, static_cast<unsigned>(CTAS), tmA, tmB, args);
+}
+
 }  // namespace
 }  // namespace tjb
 
@@ -448,5 +963,7 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
   if (M <= 16) return launch_skinny<16>(A, W, args, lda, ldw, s);
   if (M <= 32) return launch_skinny<32>(A, W, args, lda, ldw, s);
   if (M <= 64) return launch_skinny<64>(A, W, args, lda, ldw, s);
+  const int64_t tiles = ((static_cast<int64_t>(M) + 127) / 128) * ((N + 255) / 256);
+  if (tiles * 2 >= num_sms()) return launch_wide<1>(A, W, args, lda, ldw, s);
   return launch_skinny<128>(A, W, args, lda, ldw, s);
 }
