@@ -397,8 +397,8 @@ int tjb_forward_small(const tjb_small_layer* layers, int L, const float* lnf_w,
  *
  * tjb_quantize_blocks: x [rows, K] (in_dtype f32, f16 or bf16; rows ldx
  * elements apart) -> q [rows, K] e4m3 and scales [rows, ceil(K/128)], both
- * contiguous.  K % 16 == 0, ldx % 4 == 0; x aligned to four elements, q to
- * 16 bytes.  m_tiles (nullable) as in tjb_row_tiles: rows of unlisted tiles
+ * contiguous.  K % 16 == 0; x, its rows and q start on 16-byte boundaries.
+ * m_tiles (nullable) as in tjb_row_tiles: rows of unlisted tiles
  * are neither read nor written.
  * tjb_quantize_weight_blocks: w [N, K] (rows ldw elements apart) ->
  * q [N, K] and scales [ceil(N/128), ceil(K/128)]; same rules.

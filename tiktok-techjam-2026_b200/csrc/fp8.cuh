@@ -23,38 +23,68 @@ constexpr int kLiveTileRows = 128;  // rows per entry of a live-tile list
 // an integer maximum propagates both.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-__device__ __forceinline__ uint32_t abs_bits4(float4 v) {
-  return max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
+// max(|a|, |b|) that propagates NaN.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
 }
 
-// Scale of a block whose largest magnitude has these bits.
-__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
-  const float s = __uint_as_float(amax_bits) / 448.f;
-  return s < 1.17549435e-38f ? 1.17549435e-38f : s;  // a NaN stays a NaN
+__device__ __forceinline__ float max_abs4(float4 v) {
+  return max_abs(max_abs(v.x, v.y), max_abs(v.z, v.w));
 }
 
-// v / s correctly rounded, given inv = 1 / s correctly rounded: the quotient
-// from the reciprocal, corrected once by its remainder (Markstein, IBM J. Res.
-// Dev. 34, 1990).  The plain product v * inv moves about one value in 10^6
-// across a rounding border of the 8-bit type, and a full division costs about
-// three times these three operations.  With s NaN or infinite: NaN.
+// Largest magnitude over the warp (NaN included).
+__device__ __forceinline__ float warp_max_abs(float v) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(v)));
+}
+
+// v / s given inv = 1 / s: the quotient from the reciprocal, corrected once by
+// its remainder (Markstein, IBM J. Res. Dev. 34, 1990).  The plain product
+// v * inv moves about one value in 10^6 across a rounding border of the 8-bit
+// type, and full divisions bound the memory-bound kernels here by their
+// instructions (a 65536 x 4096 norm: 540 us against 461).  With s NaN or
+// infinite: NaN.
 __device__ __forceinline__ float div_by(float v, float s, float inv) {
   const float q = v * inv;
   return fmaf(fmaf(-q, s, v), inv, q);
 }
 
+// 1 / s for s in [2^-126, 2^126): the hardware's approximation and one step
+// of Newton's iteration.
+__device__ __forceinline__ float reciprocal(float s) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return fmaf(fmaf(-s, r, 1.f), r, r);
+}
+
+// Scale of a block whose largest magnitude is amax.
+__device__ __forceinline__ float block_scale(float amax) {
+  const float s = div_by(amax, 448.f, 1.f / 448.f);
+  if (abs_bits(amax) >= 0x7f800000u) return amax;  // NaN or infinite
+  return fmaxf(s, 1.17549435e-38f);
+}
+
 // Four e4m3 bytes of v / s, the first in the lowest byte (inv = 1 / s).
 __device__ __forceinline__ uint32_t quantize4(const float* v, float s, float inv) {
-  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(
-      make_float2(div_by(v[0], s, inv), div_by(v[1], s, inv)), __NV_SATFINITE, __NV_E4M3);
-  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(
-      make_float2(div_by(v[2], s, inv), div_by(v[3], s, inv)), __NV_SATFINITE, __NV_E4M3);
+  float q[4], e[4];
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {  // div_by on packed pairs
+    q[i] = v[i] * inv;
+    q[i + 1] = v[i + 1] * inv;
+    fma2v(e[i], e[i + 1], q[i], q[i + 1], -s, -s, v[i], v[i + 1]);
+    fma2v(q[i], q[i + 1], e[i], e[i + 1], inv, inv, q[i], q[i + 1]);
+  }
+  const __nv_fp8x2_storage_t lo =
+      __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi =
+      __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 
-__device__ __forceinline__ uint32_t quantize4(float4 v, float s) {
+__device__ __forceinline__ uint32_t quantize4(float4 v, float s, float inv) {
   const float f[4] = {v.x, v.y, v.z, v.w};
-  return quantize4(f, s, __frcp_rn(s));
+  return quantize4(f, s, inv);
 }
 
 // Four consecutive elements of a row: raw as loaded (16 or 8 bytes), widened

@@ -338,10 +338,10 @@ __global__ void __launch_bounds__(SkinnyCfg<BT>::kThreads)
       }
       if (args.out_dtype == TJB_E4M3) {
         if (n >= args.N) v = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float s = block_scale(__reduce_max_sync(0xffffffffu, abs_bits4(v)));
+        const float s = block_scale(warp_max_abs(max_abs4(v)));
         if (n < args.N)
           *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(args.C) + m * args.ldc + n) =
-              quantize4(v, s);
+              quantize4(v, s, reciprocal(s));
         if (lane == 0)
           args.c_scales[m * ((args.N + kQBlock - 1) / kQBlock) + n_blk] = s;
       } else if (n < args.N) {
@@ -801,11 +801,11 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
       if (row >= args.M) continue;
       const int cols = min(args.N - n0, 128);
       if (args.out_dtype == TJB_E4M3) {
-        uint32_t top = 0;
+        float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < 128; ++j) top = max(top, abs_bits(sum[j]));
+        for (int j = 0; j < 128; ++j) top = max_abs(top, sum[j]);
         const float s = block_scale(top);
-        const float inv = __frcp_rn(s);
+        const float inv = reciprocal(s);
         args.c_scales[row * ((args.N + kQBlock - 1) / kQBlock) + n0 / kQBlock] = s;
         uint8_t* dst = static_cast<uint8_t*>(args.C) + row * args.ldc + n0;
 #pragma unroll

@@ -9,12 +9,20 @@
 // 4 (i TPR + t) .. +3: the 32 lanes of a warp hold 128 consecutive, aligned
 // columns of a chunk, which is exactly one scale block, so its amax is one
 // warp-wide integer maximum of values already in registers.
+#include <type_traits>
+
 #include "fp8.cuh"
 
 namespace tjb {
 namespace {
 
-constexpr int kRmsChunks = 8;  // row chunks a thread holds: d <= 32 TPR
+// Row chunks a thread holds (d <= 16 TPR).  Four keep a thread at about 40
+// registers: what counts is the bytes that all threads of an SM have in
+// flight, and eight chunks, weights fetched ahead of the sum, or a persistent
+// block with the next row in flight all lost more by the threads they cost
+// (16384 x 4096, bf16 inputs, 8-bit output: 87 us; 117 with early weights, 124
+// persistent; 65536 x 4096 fp32 + fp16: 432, 436 and 610 us).
+constexpr int kRmsChunks = 4;
 
 // Sum over the TPR threads of a row; every thread of the block calls it.
 template <int TPR>
@@ -34,13 +42,14 @@ __device__ __forceinline__ float rms_row_sum(float v, float* scratch) {
 }
 
 // kDelta: 0 none, 1 fp32, 2 sixteen bits.
-template <int TPR, int BLOCK, bool kRes16, int kDelta>
-__global__ void __launch_bounds__(BLOCK)
+template <int TPR, bool kRes16, int kDelta>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     add_rmsnorm_kernel(const void* res, const void* delta, void* res_out, void* out,
                        float* __restrict__ out_scales, const float* __restrict__ w, int rows,
                        int d, float eps, int res_dtype, int delta_dtype, int out_dtype,
                        const uint8_t* __restrict__ row_mask,
                        const int32_t* __restrict__ m_tiles) {
+  constexpr int BLOCK = TPR < 256 ? 256 : TPR;
   constexpr int kRowsPerBlock = BLOCK / TPR;
   __shared__ float scratch[BLOCK / 32];
   const int t = threadIdx.x % TPR;
@@ -105,9 +114,10 @@ __global__ void __launch_bounds__(BLOCK)
       }
     }
     if (out_dtype == TJB_E4M3) {
-      const float s = block_scale(__reduce_max_sync(0xffffffffu, abs_bits4(y)));
+      const float s = block_scale(warp_max_abs(max_abs4(y)));
       if (col < d)
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + base + col) = quantize4(y, s);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + base + col) =
+            quantize4(y, s, reciprocal(s));
       if ((t & 31) == 0) out_scales[row * kb_count + kb] = s;
     } else if (col < d) {
       store4(out, out_dtype, base + col, y);
@@ -143,19 +153,29 @@ extern "C" int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out
   if (!device_ok()) return TJB_ERR_NO_DEVICE;
   if (rows == 0) return TJB_OK;
   const int64_t n = m_tiles ? (rows + kLiveTileRows - 1) / kLiveTileRows * kLiveTileRows : rows;
-  auto go = [&](auto kern, int block, int per_block) {
-    return launch_kernel(kern, dim3(static_cast<unsigned>((n + per_block - 1) / per_block)),
-                         dim3(block), 0, reinterpret_cast<cudaStream_t>(stream), res, delta,
-                         res_out, out, out_scales, w, static_cast<int>(rows), d, eps, res_dtype,
-                         delta_dtype, out_dtype, row_mask, m_tiles);
+  // Threads per row: enough for the row (16 columns each); with few rows, up
+  // to one chunk of four columns each, since then the latency of a row counts
+  // and not the number of threads.
+  int tpr = 32;
+  while (16 * tpr < d || (tpr < 1024 && 4 * tpr < d && 2 * n * tpr <= 1024 * num_sms())) tpr *= 2;
+  auto go = [&](auto tprc, auto res16, auto kdelta) {
+    constexpr int TPR = decltype(tprc)::value;
+    constexpr int block = TPR < 256 ? 256 : TPR, per_block = block / TPR;
+    return launch_kernel(add_rmsnorm_kernel<TPR, decltype(res16)::value, decltype(kdelta)::value>,
+                         dim3(static_cast<unsigned>((n + per_block - 1) / per_block)), dim3(block),
+                         0, reinterpret_cast<cudaStream_t>(stream), res, delta, res_out, out,
+                         out_scales, w, static_cast<int>(rows), d, eps, res_dtype, delta_dtype,
+                         out_dtype, row_mask, m_tiles);
   };
   auto pick = [&](auto res16, auto kdelta) {
-    constexpr bool R = decltype(res16)::value;
-    constexpr int D = decltype(kdelta)::value;
-    if (d <= 32 * 32) return go(add_rmsnorm_kernel<32, 256, R, D>, 256, 8);
-    if (d <= 32 * 128) return go(add_rmsnorm_kernel<128, 256, R, D>, 256, 2);
-    if (d <= 32 * 256) return go(add_rmsnorm_kernel<256, 256, R, D>, 256, 1);
-    return go(add_rmsnorm_kernel<512, 512, R, D>, 512, 1);
+    switch (tpr) {
+      case 32: return go(std::integral_constant<int, 32>{}, res16, kdelta);
+      case 64: return go(std::integral_constant<int, 64>{}, res16, kdelta);
+      case 128: return go(std::integral_constant<int, 128>{}, res16, kdelta);
+      case 256: return go(std::integral_constant<int, 256>{}, res16, kdelta);
+      case 512: return go(std::integral_constant<int, 512>{}, res16, kdelta);
+      default: return go(std::integral_constant<int, 1024>{}, res16, kdelta);
+    }
   };
   auto with_delta = [&](auto res16) {
     if (!delta) return pick(res16, std::integral_constant<int, 0>{});

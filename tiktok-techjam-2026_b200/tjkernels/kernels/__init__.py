@@ -449,24 +449,30 @@ def _blocks(n: int) -> int:
 
 def _need_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
     """The CUDA device that every given tensor is on."""
-    _need_cuda(first, *others)
     device = first.device
     for t in others:
         if t is not None and t.device != device:
+            _need_cuda(first, t)
             raise ValueError(f"tensors on {device} and {t.device}: one call runs on one device")
+    if device.type != "cuda":
+        _need_cuda(first)
     return device
 
 
 def _launch(what: str, device: torch.device, *args) -> None:
     """Call C entry point ``what`` with ``args`` and the current stream of
-    ``device``, which need not be the current device."""
+    ``device``, which need not be the current device.  (The raw stream handle:
+    building a Stream object costs as much as the launch.)"""
     fn = getattr(_lib.lib(), what)
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, _stream(device))
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            status = fn(*args, _stream(device))
-    _lib.check(status, what)
+            status = fn(*args, stream)
+    if status:
+        _lib.check(status, what)
 
 
 def _rows(t: torch.Tensor, unit: int) -> Tuple[torch.Tensor, int]:
@@ -501,10 +507,10 @@ def quantize_blocks(x: torch.Tensor, m_tiles: Optional[torch.Tensor] = None
     code = _code(x.dtype)
     r, k = x.shape
     _check_tiles(m_tiles, r)
-    q = torch.empty((r, k), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty((r, _blocks(k)), dtype=torch.float32, device=device)
+    q = x.new_empty((r, k), dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((r, _blocks(k)), dtype=torch.float32)
     if r:
-        x, ld = _rows(x, 4)
+        x, ld = _rows(x, 16 // x.element_size())
         _launch("tjb_quantize_blocks", device, _ptr(x), ld, code, _ptr(q), _ptr(scales), r, k,
                 _ptr(m_tiles))
     return q, scales
@@ -519,10 +525,10 @@ def quantize_weight_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]
         raise ValueError("w must be [N, K]")
     code = _code(w.dtype)
     n, k = w.shape
-    q = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty((_blocks(n), _blocks(k)), dtype=torch.float32, device=device)
+    q = w.new_empty((n, k), dtype=torch.float8_e4m3fn)
+    scales = w.new_empty((_blocks(n), _blocks(k)), dtype=torch.float32)
     if n:
-        w, ld = _rows(w, 4)
+        w, ld = _rows(w, 16 // w.element_size())
         _launch("tjb_quantize_weight_blocks", device, _ptr(w), ld, code, _ptr(q), _ptr(scales),
                 n, k)
     return q, scales
@@ -574,10 +580,10 @@ def fused_add_rmsnorm(
     scales = None
     if out_dtype == torch.float8_e4m3fn:
         out_code = _lib.TJB_E4M3
-        scales = torch.empty((rows, _blocks(d)), dtype=torch.float32, device=device)
+        scales = weight.new_empty((rows, _blocks(d)))
     else:
         out_code = _code(out_dtype)
-    out = torch.empty((rows, d), dtype=out_dtype, device=device)
+    out = residual.new_empty((rows, d), dtype=out_dtype)
     res_out = None
     if write_residual and delta is not None:
         if residual_out is None:
@@ -634,11 +640,11 @@ def gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales:
     scales = None
     if out_dtype == torch.float8_e4m3fn:
         out_code, unit = _lib.TJB_E4M3, 16
-        scales = torch.empty((m, _blocks(n)), dtype=torch.float32, device=device)
+        scales = a_scales.new_empty((m, _blocks(n)))
     else:
         out_code, unit = _code(out_dtype), 8
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=device)
+        out = a.new_empty((m, n), dtype=out_dtype)
     elif out.shape != (m, n) or out.dtype != out_dtype or (m and n > 1 and out.stride(1) != 1):
         raise ValueError("out must be an [M, N] tensor of out_dtype with consecutive columns")
     if m:
