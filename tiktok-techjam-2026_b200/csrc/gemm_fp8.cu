@@ -8,7 +8,7 @@
 // read back, scale and add to fp32 sums in registers while the tensor core
 // works on the next block.
 //
-// Tokens per tile, BT = 16 .. 128: the weights are the MMA's 128-row operand
+// Up to 64 tokens, in tiles of BT = 16, 32 or 64: the weights are the MMA's 128-row operand
 // (TMEM lane = output column n) and the tokens its N operand, so a few tokens
 // cost a narrow MMA and not a padded one.  The k-blocks of a tile are divided
 // over the CTAs of a cluster (so that enough SMs stream the weights), whose
@@ -17,8 +17,8 @@
 //   warp 0      TMA producer: 128 x 128-byte weight and BT x 128-byte token
 //               tiles (128-byte swizzle; one k-block) into a stage ring
 //   warp 1      owns tensor memory, issues the MMAs
-//   warps 2..   scaling: one TMEM lane (one n) per thread, BT tokens (64 of
-//               128 in each of two warp groups)
+//   warps 2..   scaling: one TMEM lane (one n) per thread, BT tokens (32 of
+//               64 in each of two warp groups)
 #include <mutex>
 
 #include "fp8.cuh"
@@ -41,6 +41,7 @@ struct GemmF8Args {
   int M, N, K, ldc;
   int out_dtype, act;
   int splits;  // CTAs per cluster (a power of two)
+  int first_tile, end_tile;  // wide kernel: the tiles of this launch
   bool wide_stores;  // C and its rows start on 32-byte boundaries
 };
 
@@ -49,10 +50,10 @@ struct SkinnyCfg {
   static constexpr int kGroups = BT >= 64 ? 2 : 1;  // scaling warp groups
   static constexpr int kCols = BT / kGroups;        // tokens per scaling thread
   static constexpr int kThreads = 64 + 128 * kGroups;
-  static constexpr int kAccs = BT == 128 ? 2 : 4;  // TMEM accumulators in flight
+  static constexpr int kAccs = 4;                   // TMEM accumulators in flight
   static constexpr uint32_t kTmemCols = kAccs * BT;
-  // Below 128 tokens two CTAs fit an SM (twice the loads in flight).
-  static constexpr int kStages = BT == 16 ? 5 : (BT == 64 ? 3 : 4);
+  // Two CTAs fit an SM.
+  static constexpr int kStages = BT == 16 ? 5 : (BT == 32 ? 4 : 3);
   static constexpr uint32_t kWBytes = kF8Lanes * kF8BK;
   static constexpr uint32_t kXBytes = BT * kF8BK;
   static constexpr uint32_t kExBytes = BT * kF8Lanes * 4;  // partial sums from the cluster
@@ -84,9 +85,43 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 template <int kThreads>
 __device__ __forceinline__ void scaling_warps_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+}
+
+// Columns n .. n + 3 of token m (one warp holds 128 columns, this lane four):
+// bias, activation, rounding, store.  With an 8-bit output the warp's columns
+// are one block.
+__device__ __forceinline__ void finish4(const GemmF8Args& args, float4 v, float4 bias, int64_t m,
+                                        int n, int lane) {
+  v.x += bias.x;
+  v.y += bias.y;
+  v.z += bias.z;
+  v.w += bias.w;
+  if (args.act == 1) {
+    gelu_erf2(v.x, v.y);
+    gelu_erf2(v.z, v.w);
+  }
+  if (args.out_dtype == TJB_E4M3) {
+    if (n >= args.N) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float s = block_scale(warp_max_abs(max_abs4(v)));
+    if (n < args.N)
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(args.C) + m * args.ldc + n) =
+          quantize4(v, s, reciprocal(s));
+    if (lane == 0) args.c_scales[m * ((args.N + kQBlock - 1) / kQBlock) + n / kQBlock] = s;
+  } else if (n < args.N) {
+    store4(args.C, args.out_dtype, m * args.ldc + n, v);
+  }
 }
 
 template <int BT>
@@ -143,9 +178,6 @@ __global__ void __launch_bounds__(SkinnyCfg<BT>::kThreads)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  griddep_wait();
-  griddep_launch_dependents();
-
   // This cluster's tile: 128 output columns, BT tokens from t0.
   constexpr int kPerLive = kLiveTileRows / BT;
   const int t_tiles = args.m_tiles != nullptr
@@ -153,6 +185,17 @@ __global__ void __launch_bounds__(SkinnyCfg<BT>::kThreads)
                           : (args.M + BT - 1) / BT;
   const int n_blk = tile / t_tiles;
   const int tt = tile - n_blk * t_tiles;
+  const int kb_count = (args.K + kF8BK - 1) / kF8BK;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * kb_count / splits);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * kb_count / splits);
+  // The first weight tiles start for L2 while the previous kernel drains (L2
+  // holds whatever that kernel may still write to them).
+  if (warp == 0 && lane == 0)
+    for (int i = kb0; i < kb1 && i < kb0 + kStages; ++i)
+      tma_prefetch_2d(&tmW, i * kF8BK, n_blk * kF8Lanes);
+  __syncwarp();
+  griddep_wait();
+  griddep_launch_dependents();
   int t0 = tt * BT;
   bool live = true;
   if (args.m_tiles != nullptr) {
@@ -161,9 +204,6 @@ __global__ void __launch_bounds__(SkinnyCfg<BT>::kThreads)
     if (live) t0 = __ldg(args.m_tiles + 1 + li) * kLiveTileRows + (tt % kPerLive) * BT;
   }
   const int tokens = live ? min(BT, args.M - t0) : 0;  // may be <= 0: nothing to do
-  const int kb_count = (args.K + kF8BK - 1) / kF8BK;
-  const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * kb_count / splits);
-  const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * kb_count / splits);
   const int n_kb = tokens > 0 ? kb1 - kb0 : 0;
 
   if (warp == 0) {
@@ -326,27 +366,7 @@ __global__ void __launch_bounds__(SkinnyCfg<BT>::kThreads)
         v.z += u.z;
         v.w += u.w;
       }
-      v.x += bias.x;
-      v.y += bias.y;
-      v.z += bias.z;
-      v.w += bias.w;
-      if (args.act == 1) {
-        v.x = gelu_erf(v.x);
-        v.y = gelu_erf(v.y);
-        v.z = gelu_erf(v.z);
-        v.w = gelu_erf(v.w);
-      }
-      if (args.out_dtype == TJB_E4M3) {
-        if (n >= args.N) v = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float s = block_scale(warp_max_abs(max_abs4(v)));
-        if (n < args.N)
-          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(args.C) + m * args.ldc + n) =
-              quantize4(v, s, reciprocal(s));
-        if (lane == 0)
-          args.c_scales[m * ((args.N + kQBlock - 1) / kQBlock) + n_blk] = s;
-      } else if (n < args.N) {
-        store4(args.C, args.out_dtype, m * args.ldc + n, v);
-      }
+      finish4(args, v, bias, m, n, lane);
     }
   }
   tc_fence_before();
@@ -359,13 +379,13 @@ __global__ void __launch_bounds__(SkinnyCfg<BT>::kThreads)
 }
 
 std::mutex g_f8_mu;
-bool g_f8_ready[64][4];
+bool g_f8_ready[64][3];
 
 template <int BT>
 int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
                   cudaStream_t stream) {
   using Cfg = SkinnyCfg<BT>;
-  constexpr int kSlot = BT == 16 ? 0 : BT == 32 ? 1 : BT == 64 ? 2 : 3;
+  constexpr int kSlot = BT == 16 ? 0 : BT == 32 ? 1 : 2;
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return TJB_ERR_NO_DEVICE;
@@ -389,11 +409,13 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
                                     (kLiveTileRows / BT)
                               : (args.M + BT - 1) / BT;
   const int64_t tiles = t_tiles * ((args.N + kF8Lanes - 1) / kF8Lanes);
-  // As many CTAs per tile as the SMs have room for, at most one per k-block.
-  const int64_t slots = static_cast<int64_t>(num_sms()) * (BT < 128 ? 2 : 1);
+  // As many CTAs per tile as the SMs have room for, at most one per k-block;
+  // more than four lose more in their meeting than they gain (M16 N4096 K4096:
+  // 7.2 us with four, 8.0 with eight).
+  const int64_t slots = static_cast<int64_t>(num_sms()) * 2;
   const int kb_count = (args.K + kF8BK - 1) / kF8BK;
   args.splits = 1;
-  while (args.splits < 8 && 2 * args.splits <= kb_count && tiles * 2 * args.splits <= slots)
+  while (args.splits < 4 && 2 * args.splits <= kb_count && tiles * 2 * args.splits <= slots)
     args.splits *= 2;
   const int64_t grid = tiles * args.splits;
   if (grid > 2147483647) return TJB_ERR_BAD_SHAPE;
@@ -403,14 +425,12 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
 }
 
 // ------------------------------------------------------------------------
-// Many tokens: 128 x 256 tiles of C per CTA (with CTAS = 2 a CTA pair shares
-// the MMAs of a 256 x 256 tile, CTA r holding token rows 128 r .. of it and
-// 128 of its 256 weight rows).  Here the tokens are the MMA's rows: a thread
-// owns one token and 128 consecutive output columns, which is one weight
+// More tokens: 128 x 256 tiles of C.  Here the tokens are the MMA's rows: a
+// thread owns one token and 128 consecutive output columns, which is one weight
 // block (one scale product per k-block) and one output block (its 8-bit scale
 // needs no exchange).  Persistent, 384 threads:
 //   warp 0        TMA producer
-//   warp 1        MMA issuer (leader CTA): per k-block four K = 32 MMAs into
+//   warp 1        MMA issuer: per k-block four K = 32 MMAs into
 //                 one of two 256-column TMEM accumulators
 //   warps 2, 3    products sa[m, kb] sw[n / 128, kb] of the tile's rows, eight
 //                 k-blocks at a time, a ring slot ahead of their use
@@ -423,40 +443,28 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
 // warp).  What bounds it is the chain MMA -> barrier -> scaling -> barrier ->
 // MMA over the two accumulators: every barrier operation, load and spilled
 // register in the k-loop adds to it.  The scaling threads need the registers
-// that warps 0-3 give up (128 x 72 + 256 x 216 = 384 x 168 at launch).
-template <int CTAS>
+// that warps 0-3 give up (128 x 72 + 256 x 216 = 384 x 168 at launch).  Loads,
+// MMAs and sums together also draw the board's power limit (clocks near 1.45
+// GHz at M16384 N4096 K16384).  A CTA-pair form (two SMs on one 256 x 256
+// tile, a third less L2 traffic) ran the long products as fast and those with
+// K = 1024 a tenth slower: its hand-backs cross SMs.
+//
+// kSplit: the tile's k-blocks are divided over the CTAs of a cluster, for
+// products with too few tiles to fill the SMs.  Each CTA ends with fp32 sums of
+// the whole tile; CTA k finishes rows k * 128 / c ... of it, reading the other
+// CTAs' sums through distributed shared memory and adding them in a fixed
+// order.
 struct WideCfg {
-  static constexpr int kStages = CTAS == 2 ? 6 : 4;
+  static constexpr int kStages = 4;
   static constexpr int kThreads = 384;
-  static constexpr int kBRows = 256 / CTAS;       // weight rows a CTA holds per stage
   static constexpr uint32_t kABytes = 128 * kF8BK;
-  static constexpr uint32_t kBBytes = kBRows * kF8BK;
+  static constexpr uint32_t kBBytes = 256 * kF8BK;
   static constexpr uint32_t kTmemCols = 512;      // two 256-column accumulators
   static constexpr int kChunk = 8;                // k-blocks of scale products per ring slot
   static constexpr uint32_t kScaleBytes = 2 * kChunk * 256 * 4;
   static constexpr uint32_t kSmemBytes =
       1024 + kStages * (kABytes + kBBytes) + kScaleBytes + 256;
 };
-
-__device__ __forceinline__ void umma_e4m3_pair_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                                 uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Arrive on an mbarrier of another CTA of the cluster to hand back tensor
-// memory that this thread has finished reading.  The reads are complete and
-// ordered by tcgen05.fence, and no other memory is handed over, so the arrive
-// needs no release at cluster scope (whose fence, once per k-block, made the
-// kernel wait 4x the MMA time: 8192 x 4096 x 4096 328 us).
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t remote_bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
-}
 
 template <int kRegs>
 __device__ __forceinline__ void regs_dec() {
@@ -484,23 +492,6 @@ __device__ __forceinline__ void store32(void* dst, const uint32_t (&w)[8], int c
   if (cols >= 2 * per16) p[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-template <int CTAS>
-__device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                     uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CTAS == 2)
-    umma_e4m3_pair_w(d_tmem, adesc, bdesc, idesc, accumulate);
-  else
-    umma_e4m3_w(d_tmem, adesc, bdesc, idesc, accumulate);
-}
-
-template <int CTAS>
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  if constexpr (CTAS == 2)
-    umma_commit_pair_w(bar, 0x3);
-  else
-    umma_commit_w(bar);
-}
-
 // sum[0..15] += s * p[0..15]
 __device__ __forceinline__ void add_scaledN(float* sum, const uint32_t* p, float s) {
 #pragma unroll
@@ -509,13 +500,51 @@ __device__ __forceinline__ void add_scaledN(float* sum, const uint32_t* p, float
           sum[j + 1]);
 }
 
-template <int CTAS>
-__global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
+// The rows of a split tile that CTA `rank` of C finishes, of which warp `quad`
+// of a half takes a quarter: the C parts of each are summed (32 loads in
+// flight) and finished.
+template <int C>
+__device__ __forceinline__ void pull_rows(const GemmF8Args& args, uint32_t half_at, int rank,
+                                          int quad, int64_t m0, int n0, int lane) {
+  constexpr int kRows = 32 / C;                   // per warp
+  constexpr int kGroup = kRows < 8 ? kRows : 8;   // at a time
+  const int n = n0 + lane * 4;
+  float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (args.bias != nullptr && n < args.N)
+    bias = __ldg(reinterpret_cast<const float4*>(args.bias + n));
+#pragma unroll 1
+  for (int g = 0; g < kRows; g += kGroup) {
+    const int row0 = rank * (128 / C) + quad * kRows + g;
+    float4 part[kGroup][C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const uint32_t from = map_to_rank(half_at, static_cast<uint32_t>(c));
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i)
+        part[i][c] = ld_cluster_v4(
+            from + static_cast<uint32_t>((row0 + i) * 512 + (lane ^ ((row0 + i) & 31)) * 16));
+    }
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      float4 v = part[i][0];
+#pragma unroll
+      for (int c = 1; c < C; ++c) {
+        v.x += part[i][c].x;
+        v.y += part[i][c].y;
+        v.z += part[i][c].z;
+        v.w += part[i][c].w;
+      }
+      if (m0 + row0 + i < args.M) finish4(args, v, bias, m0 + row0 + i, n, lane);  // warp-uniform
+    }
+  }
+}
+
+template <bool kSplit>
+__global__ void __launch_bounds__(WideCfg::kThreads, 1)
     gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmA,
                          const __grid_constant__ CUtensorMap tmB,
                          const GemmF8Args args) {
-  using Cfg = WideCfg<CTAS>;
-  constexpr bool kPair = CTAS == 2;
+  using Cfg = WideCfg;
   constexpr int kStages = Cfg::kStages, kChunk = Cfg::kChunk;
   constexpr int BN = 256;
   extern __shared__ uint8_t smem_raw[];
@@ -524,10 +553,10 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
   uint8_t* sA = smem;
   uint8_t* sB = sA + kStages * Cfg::kABytes;
   float* sScale = reinterpret_cast<float*>(sB + kStages * Cfg::kBBytes);  // [slot][k-block][half][row]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sScale + 2 * kChunk * 256);  // leader's are used
+  uint64_t* full = reinterpret_cast<uint64_t*>(sScale + 2 * kChunk * 256);
   uint64_t* empty = full + kStages;
   uint64_t* tfull = empty + kStages;
-  uint64_t* tempty = tfull + 2;  // leader's are used
+  uint64_t* tempty = tfull + 2;
   uint64_t* sfull = tempty + 2;
   uint64_t* sempty = sfull + 2;
   uint64_t* drain = sempty + 2;
@@ -535,17 +564,18 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = kPair ? cluster_ctarank() : 0u;  // 0: the leader, which issues the MMAs
+  const int splits = kSplit ? args.splits : 1;
+  const int rank = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);   // the leader's expect-tx arrival + both CTAs' bytes
-      mbar_init(&empty[s], 1);  // one commit of the leader's MMAs to both CTAs
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 8 * CTAS);  // eight scaling warps of each CTA
-      mbar_init(&sfull[b], 2);  // warps 2 and 3
+      mbar_init(&tempty[b], 8);  // the scaling warps
+      mbar_init(&sfull[b], 2);   // warps 2 and 3
       mbar_init(&sempty[b], 8);  // the scaling warps
     }
     mbar_init(drain, 1);
@@ -555,75 +585,48 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
     prefetch_tmap(&tmB);
   }
   if (warp == 1) {
-    if constexpr (kPair) {
-      tmem_alloc_pair(tmem_slot, Cfg::kTmemCols);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(tmem_slot, Cfg::kTmemCols);
-      tmem_relinquish();
-    }
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
   }
   __syncwarp();
   tc_fence_before();
-  // Both CTAs' barriers are initialised and their tensor memory allocated
-  // before either signals the other.
-  if constexpr (kPair)
-    cluster_sync();
-  else
-    __syncthreads();
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();
   griddep_launch_dependents();
   const int num_m = args.m_tiles != nullptr ? __ldg(args.m_tiles) : (args.M + 127) / 128;
-  const int num_mp = (num_m + CTAS - 1) / CTAS;
   const int num_n = (args.N + BN - 1) / BN;
   const int num_k = (args.K + kF8BK - 1) / kF8BK;
-  const int num_tiles = num_mp * num_n;
-  const int first = static_cast<int>(blockIdx.x) / CTAS;
-  const int step = static_cast<int>(gridDim.x) / CTAS;
-  // This CTA's 128 token rows of pair tile t.  A pair whose second 128-row
-  // tile does not exist loads the first one's rows again (the MMA needs both
-  // halves) and its second CTA stores nothing.
+  // Tiles first, first + step, ... below end; k-blocks [k0, k1) of each.
+  const int end = min(num_m * num_n, args.end_tile);
+  const int first = args.first_tile + static_cast<int>(blockIdx.x) / splits;
+  const int step = kSplit ? end : static_cast<int>(gridDim.x);  // (kSplit: one tile)
+  const int k0 = kSplit ? rank * num_k / splits : 0;
+  const int k1 = kSplit ? (rank + 1) * num_k / splits : num_k;
   auto coords = [&](int t, int& m_blk, int& n_blk) {
-    int mp;
-    tile_coords(t, num_mp, num_n, mp, n_blk);
-    int mt = CTAS * mp + static_cast<int>(rank);
-    const bool has = mt < num_m;
-    if (!has) mt = CTAS * mp;
-    m_blk = args.m_tiles != nullptr ? __ldg(args.m_tiles + 1 + mt) : mt;
-    return has;
+    tile_coords(t, num_m, num_n, m_blk, n_blk);
+    if (args.m_tiles != nullptr) m_blk = __ldg(args.m_tiles + 1 + m_blk);
   };
 
   if (warp < 4) {
     regs_dec<72>();
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ producer
-      const uint32_t full_leader = kPair ? map_to_rank(smem_u32(full), 0) : 0u;
       int stage = 0;
       uint32_t phase = 0, issued = 0, last_parity = 0;
       bool ok = true;
-      for (int t = first; ok && t < num_tiles; t += step) {
+      for (int t = first; ok && t < end; t += step) {
         int m_blk, n_blk;
         coords(t, m_blk, n_blk);
-        for (int kb = 0; kb < num_k; ++kb) {
+        for (int kb = k0; kb < k1; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
             ok = false;
             break;
           }
-          if (rank == 0)
-            mbar_arrive_expect_tx(&full[stage], CTAS * (Cfg::kABytes + Cfg::kBBytes));
-          uint8_t* a = sA + stage * Cfg::kABytes;
-          uint8_t* b = sB + stage * Cfg::kBBytes;
-          const int brow = n_blk * BN + static_cast<int>(rank) * Cfg::kBRows;
-          if constexpr (kPair) {
-            const uint32_t bar = full_leader + static_cast<uint32_t>(stage) * 8u;
-            tma_load_2d_pair(a, &tmA, bar, kb * kF8BK, m_blk * 128);
-            tma_load_2d_pair(b, &tmB, bar, kb * kF8BK, brow);
-          } else {
-            tma_load_2d(a, &tmA, &full[stage], kb * kF8BK, m_blk * 128);
-            tma_load_2d(b, &tmB, &full[stage], kb * kF8BK, brow);
-          }
+          mbar_arrive_expect_tx(&full[stage], Cfg::kABytes + Cfg::kBBytes);
+          tma_load_2d(sA + stage * Cfg::kABytes, &tmA, &full[stage], kb * kF8BK, m_blk * 128);
+          tma_load_2d(sB + stage * Cfg::kBBytes, &tmB, &full[stage], kb * kF8BK, n_blk * BN);
           issued |= 1u << stage;
           last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
           if (++stage == kStages) {
@@ -632,21 +635,20 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
           }
         }
       }
-      // Every load this CTA issued has landed once the MMAs that read it
-      // have released its stage (the loads count on the leader's barrier).
+      // Every load has landed before the CTA may release its memory.
       for (int s = 0; s < kStages; ++s)
-        if ((issued >> s) & 1u) mbar_wait_drain(&empty[s], (last_parity >> s) & 1u);
-    } else if (warp == 1 && rank == 0) {
-      // ---------------------------------------------- MMA issuer (leader only)
-      constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, BN);
+        if ((issued >> s) & 1u) mbar_wait_drain(&full[s], (last_parity >> s) & 1u);
+    } else if (warp == 1) {
+      // ---------------------------------------------------------- MMA issuer
+      constexpr uint32_t idesc = idesc_e4m3(128, BN);
       int stage = 0;
       uint32_t phase = 0, it = 0;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
       };
-      for (int t = first; ok && t < num_tiles; t += step) {
-        for (int kb = 0; kb < num_k; ++kb, ++it) {
+      for (int t = first; ok && t < end; t += step) {
+        for (int kb = k0; kb < k1; ++kb, ++it) {
           const uint32_t acc = it & 1;
           if (!wait(&full[stage], phase) || !wait(&tempty[acc], ((it >> 1) & 1) ^ 1)) {
             ok = false;
@@ -657,20 +659,17 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
           const uint32_t b0 = smem_u32(sB + stage * Cfg::kBBytes);
 #pragma unroll
           for (int k = 0; k < kF8BK / 32; ++k)
-            umma<CTAS>(tmem_base + acc * BN, sdesc_sw128(a0 + k * 32, 16, 1024),
-                       sdesc_sw128(b0 + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
-          commit<CTAS>(&tfull[acc]);
-          commit<CTAS>(&empty[stage]);
+            umma_e4m3_w(tmem_base + acc * BN, sdesc_sw128(a0 + k * 32, 16, 1024),
+                        sdesc_sw128(b0 + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
+          umma_commit_w(&tfull[acc]);
+          umma_commit_w(&empty[stage]);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      if constexpr (kPair)
-        umma_commit_pair_w(drain, 0x1);
-      else
-        umma_commit_w(drain);
+      umma_commit_w(drain);
       mbar_wait_drain(drain, 0);
     } else if (warp >= 2) {
       // --------------------------------------------------------- scale products
@@ -682,7 +681,7 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
                        (reinterpret_cast<uintptr_t>(args.a_scales) & 15u) == 0;
       uint32_t c = 0;
       bool ok = true;
-      for (int t = first; ok && t < num_tiles; t += step) {
+      for (int t = first; ok && t < end; t += step) {
         int m_blk, n_blk;
         coords(t, m_blk, n_blk);
         const int64_t row = static_cast<int64_t>(m_blk) * 128 + r;
@@ -693,9 +692,9 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
             args.a_scales + min(row + 32, static_cast<int64_t>(args.M - 1)) * args.as_row;
         const float* w0 = args.w_scales + static_cast<int64_t>(2 * n_blk) * num_k;
         const float* w1 = 2 * n_blk + 1 < num_nb ? w0 + num_k : w0;
-        for (int kb0 = 0; ok && kb0 < num_k; kb0 += kChunk, ++c) {
+        for (int kb0 = k0; ok && kb0 < k1; kb0 += kChunk, ++c) {
           float va[kChunk], vb[kChunk], s0[kChunk], s1[kChunk];
-          if (vec && kb0 + kChunk <= num_k) {
+          if (vec && kb0 % 4 == 0 && kb0 + kChunk <= k1) {
 #pragma unroll
             for (int u = 0; u < kChunk; u += 4) {
               *reinterpret_cast<float4*>(va + u) = __ldg(reinterpret_cast<const float4*>(a0 + kb0 + u));
@@ -709,7 +708,7 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
           } else {
 #pragma unroll
             for (int u = 0; u < kChunk; ++u) {
-              const int kb = min(kb0 + u, num_k - 1);
+              const int kb = min(kb0 + u, k1 - 1);
               va[u] = __ldg(a0 + kb * args.as_blk);
               vb[u] = __ldg(a1 + kb * args.as_blk);
               s0[u] = __ldg(w0 + kb);
@@ -731,20 +730,25 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
         }
       }
     }
+    if constexpr (kSplit) {  // the scaling warps' two meetings below
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
   } else {
     regs_inc<216>();
     // ------------------------------------------------- scaling and output
     const int quad = warp & 3;         // TMEM lanes this warp may access
     const int half = (warp - 4) >> 2;  // 128-column half of the tile
     const int r = quad * 32 + lane;    // token row of the tile
-    const uint32_t tempty_leader = kPair ? map_to_rank(smem_u32(tempty), 0) : 0u;
     const uint32_t taddr0 =
         tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 128);
     uint32_t it = 0, chunk = 0;  // k-blocks and scale chunks done, over all tiles
     bool ok = true;
-    for (int t = first; ok && t < num_tiles; t += step) {
+    bool met = !kSplit;  // this warp has been at the cluster's two meetings
+    for (int t = first; ok && t < end; t += step) {
       int m_blk, n_blk;
-      const bool has_rows = coords(t, m_blk, n_blk);
+      coords(t, m_blk, n_blk);
       const int n0 = n_blk * BN + half * 128;
       // The sums start from the bias; columns past N stay exactly zero (their
       // weight rows load as zeros), as a ragged 8-bit block's scale needs.
@@ -752,7 +756,7 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
 #pragma unroll
       for (int j = 0; j < 128; j += 4) {
         float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (args.bias != nullptr && n0 + j < args.N)
+        if (!kSplit && args.bias != nullptr && n0 + j < args.N)
           b = __ldg(reinterpret_cast<const float4*>(args.bias + n0 + j));
         sum[j] = b.x;
         sum[j + 1] = b.y;
@@ -760,8 +764,8 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
         sum[j + 3] = b.w;
       }
 #pragma unroll 1
-      for (int kb = 0; kb < num_k; ++kb, ++it) {
-        const int u = kb & (kChunk - 1);
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int u = (kb - k0) & (kChunk - 1);
         if (u == 0) ok = mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag) && ok;
         const float s = sScale[((chunk & 1) * kChunk + u) * 256 + half * 128 + r];
         const uint32_t acc = it & 1;
@@ -781,21 +785,49 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (kPair)
-            mbar_arrive_remote(tempty_leader + acc * 8u);
-          else
-            mbar_arrive(&tempty[acc]);
-          if (u == kChunk - 1 || kb == num_k - 1) mbar_arrive(&sempty[chunk & 1]);
+          mbar_arrive(&tempty[acc]);
+          if (u == kChunk - 1 || kb == k1 - 1) mbar_arrive(&sempty[chunk & 1]);
         }
-        if (u == kChunk - 1 || kb == num_k - 1) ++chunk;
+        if (u == kChunk - 1 || kb == k1 - 1) ++chunk;
         add_scaledN(sum + 128 - 16, p[1], s);
       }
       ok = __all_sync(0xffffffffu, ok);
+      if constexpr (kSplit) {
+        // The sums go to this CTA's shared memory as [half][row][32 chunks of
+        // 16 bytes, chunk j at j ^ (row & 31)] (the stage ring: this thread
+        // has seen the last MMA's barrier, so nothing reads or writes it any
+        // more), and CTA k pulls rows k * 128 / c ... of every CTA's.  Neither
+        // these stores (a row per lane) nor the loads (a row per warp) meet in
+        // a bank, and every remote access is a whole 512-byte row; stored
+        // straight into the other CTA, a row per lane, the exchange of eight
+        // CTAs took 5.5 us more.
+        float4* mine = reinterpret_cast<float4*>(smem) + (half * 128 + r) * 32;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          mine[j ^ lane] =
+              make_float4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]);
+        __syncwarp();
+        cluster_sync();  // every CTA's sums are in place
+        met = true;
+        if (n0 < args.N) {
+          const int64_t m0 = static_cast<int64_t>(m_blk) * 128;
+          const uint32_t half_at = smem_u32(smem) + static_cast<uint32_t>(half * 128 * 512);
+          if (splits == 2)
+            pull_rows<2>(args, half_at, rank, quad, m0, n0, lane);
+          else if (splits == 4)
+            pull_rows<4>(args, half_at, rank, quad, m0, n0, lane);
+          else
+            pull_rows<8>(args, half_at, rank, quad, m0, n0, lane);
+        }
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while its sums are being read
+        break;
+      }
       if (!ok) break;
-      if (!has_rows || n0 >= args.N) continue;  // warp-uniform
+      if (n0 >= args.N) continue;  // warp-uniform
       if (args.act == 1) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j) sum[j] = gelu_erf(sum[j]);
+        for (int j = 0; j < 128; j += 2) gelu_erf2(sum[j], sum[j + 1]);
       }
       const int64_t row = static_cast<int64_t>(m_blk) * 128 + r;
       if (row >= args.M) continue;
@@ -838,82 +870,110 @@ __global__ void __launch_bounds__(WideCfg<CTAS>::kThreads, 1)
         }
       }
     }
+    if (!met) {  // no tile (a live-tile list with fewer): the same meetings
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
   }
 
-  // Neither CTA releases its tensor memory (or exits) while the leader's
-  // MMAs or the peer's scaling warps may still touch the pair's resources.
   __syncwarp();
   tc_fence_before();
-  if constexpr (kPair)
-    cluster_sync();
-  else
-    __syncthreads();
+  __syncthreads();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    if constexpr (kPair)
-      tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
-    else
-      tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
 }
 
-int g_f8_wide[64][2];  // co-resident clusters per device and form (0: not yet known)
+// Clusters of 1, 2, 4 and 8 CTAs that run at once, per device.
+struct WideLimits {
+  int clusters[4];
+  bool known;
+};
+WideLimits g_f8_wide[64];
 
-template <int CTAS>
-int wide_resident(int& clusters) {
+int wide_limits(WideLimits& lim) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return TJB_ERR_NO_DEVICE;
   std::lock_guard<std::mutex> lock(g_f8_mu);
-  int& known = g_f8_wide[dev][CTAS - 1];
-  if (known == 0) {
-    if (const int fs = cuda_status(cudaFuncSetAttribute(
-            gemm_fp8_wide_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-            static_cast<int>(WideCfg<CTAS>::kSmemBytes))))
-      return fs;
-    int n = num_sms();
-    if (CTAS == 2) {
+  WideLimits& l = g_f8_wide[dev];
+  if (!l.known) {
+    for (auto kern : {gemm_fp8_wide_kernel<false>, gemm_fp8_wide_kernel<true>})
+      if (const int fs = cuda_status(cudaFuncSetAttribute(
+              kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+              static_cast<int>(WideCfg::kSmemBytes))))
+        return fs;
+    l.clusters[0] = num_sms();
+    for (int i = 1; i < 4; ++i) {
       cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(2 * (num_sms() / 2));
-      cfg.blockDim = dim3(WideCfg<CTAS>::kThreads);
-      cfg.dynamicSmemBytes = WideCfg<CTAS>::kSmemBytes;
+      cfg.gridDim = dim3(static_cast<unsigned>(num_sms() >> i << i));
+      cfg.blockDim = dim3(WideCfg::kThreads);
+      cfg.dynamicSmemBytes = WideCfg::kSmemBytes;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 2;
+      attr[0].val.clusterDim.x = 1u << i;
       attr[0].val.clusterDim.y = 1;
       attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      if (const int qs = cuda_status(
-              cudaOccupancyMaxActiveClusters(&n, gemm_fp8_wide_kernel<CTAS>, &cfg)))
+      if (const int qs = cuda_status(cudaOccupancyMaxActiveClusters(
+              &l.clusters[i], gemm_fp8_wide_kernel<true>, &cfg)))
         return qs;
     }
-    known = n > 0 ? n : -1;
+    l.known = true;
   }
-  clusters = known;
-  return clusters > 0 ? TJB_OK : TJB_ERR_LAUNCH;
+  lim = l;
+  return TJB_OK;
 }
 
-template <int CTAS>
 int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
                 cudaStream_t stream) {
-  using Cfg = WideCfg<CTAS>;
-  int clusters = 0;
-  if (const int st = wide_resident<CTAS>(clusters)) return st;
+  using Cfg = WideCfg;
+  WideLimits lim;
+  if (const int st = wide_limits(lim)) return st;
   CUtensorMap tmA, tmB;
   int st = make_tmap_2d(&tmA, TJB_E4M3, A, args.K, args.M, lda, kF8BK, 128);
   if (st != TJB_OK) return st;
-  st = make_tmap_2d(&tmB, TJB_E4M3, W, args.K, args.N, ldw, kF8BK, Cfg::kBRows);
+  st = make_tmap_2d(&tmB, TJB_E4M3, W, args.K, args.N, ldw, kF8BK, 256);
   if (st != TJB_OK) return st;
   const int64_t esz = args.out_dtype == TJB_F32 ? 4 : args.out_dtype == TJB_E4M3 ? 1 : 2;
   args.wide_stores = ((reinterpret_cast<uintptr_t>(args.C) | (args.ldc * esz)) & 31) == 0;
-  const int64_t m_tiles = (static_cast<int64_t>(args.M) + 127) / 128;
-  const int64_t tiles = (m_tiles + CTAS - 1) / CTAS * ((args.N + 255) / 256);
-  if (tiles > 2147483647) return TJB_ERR_BAD_SHAPE;
-  const int n = tiles < clusters ? static_cast<int>(tiles) : clusters;
-  return launch_kernel_cluster(gemm_fp8_wide_kernel<CTAS>, dim3(CTAS * n), dim3(Cfg::kThreads),
-                               Cfg::kSmemBytes, stream, static_cast<unsigned>(CTAS), tmA, tmB, args);
+  const int64_t tiles64 =
+      (static_cast<int64_t>(args.M) + 127) / 128 * ((args.N + 255) / 256);
+  if (tiles64 > 1073741823) return TJB_ERR_BAD_SHAPE;
+  const int tiles = static_cast<int>(tiles64);
+  const int sms = lim.clusters[0];
+  const int num_k = (args.K + kF8BK - 1) / kF8BK;
+  // Whole rounds of one tile per SM, then the tiles left over with their
+  // k-blocks split over as many CTAs as run at once.  Splitting costs a second
+  // launch and the exchange, together about 4 k-blocks' time.
+  int whole = tiles / sms * sms;
+  int log2 = 0;
+  while (log2 < 3 && 2 << log2 <= num_k && tiles - whole <= lim.clusters[log2 + 1]) ++log2;
+  if (whole < tiles && (log2 == 0 || num_k - (num_k >> log2) < (whole > 0 ? 10 : 4)))
+    whole = tiles;
+  if (whole > 0) {
+    args.first_tile = 0;
+    args.end_tile = whole;
+    args.splits = 1;
+    const int grid = whole < sms ? whole : sms;
+    st = launch_kernel(gemm_fp8_wide_kernel<false>, dim3(grid), dim3(Cfg::kThreads),
+                       Cfg::kSmemBytes, stream, tmA, tmB, args);
+    if (st != TJB_OK) return st;
+  }
+  if (whole < tiles) {
+    args.first_tile = whole;
+    args.end_tile = tiles;
+    args.splits = 1 << log2;
+    st = launch_kernel_cluster(gemm_fp8_wide_kernel<true>,
+                               dim3(static_cast<unsigned>(tiles - whole) << log2),
+                               dim3(Cfg::kThreads), Cfg::kSmemBytes, stream,
+                               static_cast<unsigned>(args.splits), tmA, tmB, args);
+  }
+  return st;
 }
 
 }  // namespace
@@ -962,8 +1022,12 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
   // The narrowest tile that holds every token.
   if (M <= 16) return launch_skinny<16>(A, W, args, lda, ldw, s);
   if (M <= 32) return launch_skinny<32>(A, W, args, lda, ldw, s);
-  if (M <= 64) return launch_skinny<64>(A, W, args, lda, ldw, s);
-  const int64_t tiles = ((static_cast<int64_t>(M) + 127) / 128) * ((N + 255) / 256);
-  if (tiles * 2 >= num_sms()) return launch_wide<1>(A, W, args, lda, ldw, s);
-  return launch_skinny<128>(A, W, args, lda, ldw, s);
+  // Beyond, the 64-token form while the product is small: its parts meet
+  // faster than those of a wide tile, but a 64 x 128 tile keeps the tensor
+  // core a third as busy (N4096 K4096: M128 10.8 against 15.0 us, M256 16.1 and
+  // 16.0, M512 26.7 and 17.8; N1024 K1024: M512 7.2 and 10.9).
+  const int64_t blocks = ((static_cast<int64_t>(M) + 63) / 64) * ((N + 127) / 128) *
+                         ((K + kF8BK - 1) / kF8BK);
+  if (M <= 64 || blocks <= 28 * num_sms()) return launch_skinny<64>(A, W, args, lda, ldw, s);
+  return launch_wide(A, W, args, lda, ldw, s);
 }
