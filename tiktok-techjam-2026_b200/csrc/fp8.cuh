@@ -30,8 +30,15 @@ __device__ __forceinline__ float max_abs(float a, float b) {
   return r;
 }
 
+// max(|a|, |b|, |c|) in one instruction (sm_100), NaN propagated.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 __device__ __forceinline__ float max_abs4(float4 v) {
-  return max_abs(max_abs(v.x, v.y), max_abs(v.z, v.w));
+  return max_abs(max_abs(v.x, v.y, v.z), v.w, v.w);
 }
 
 // Largest magnitude over the warp (NaN included).
@@ -70,8 +77,13 @@ __device__ __forceinline__ uint32_t quantize4(const float* v, float s, float inv
   float q[4], e[4];
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {  // div_by on packed pairs
-    q[i] = v[i] * inv;
-    q[i + 1] = v[i + 1] * inv;
+    asm("{\n\t.reg .b64 ra, rb;\n\t"
+        "mov.b64 ra, {%2, %3};\n\t"
+        "mov.b64 rb, {%4, %4};\n\t"
+        "mul.rn.f32x2 ra, ra, rb;\n\t"
+        "mov.b64 {%0, %1}, ra;\n\t}"
+        : "=f"(q[i]), "=f"(q[i + 1])
+        : "f"(v[i]), "f"(v[i + 1]), "f"(inv));
     fma2v(e[i], e[i + 1], q[i], q[i + 1], -s, -s, v[i], v[i + 1]);
     fma2v(q[i], q[i + 1], e[i], e[i + 1], inv, inv, q[i], q[i + 1]);
   }
@@ -87,40 +99,35 @@ __device__ __forceinline__ uint32_t quantize4(float4 v, float s, float inv) {
   return quantize4(f, s, inv);
 }
 
-// gelu_erf (common.cuh) of a pair, by the same formula arranged for fewer
-// instructions: with h(u) as there (u = |x| / sqrt 2),
-//   GELU(x) = max(x, 0) - |x| h(u) / 2,
-// the factor -1/2 folded into the polynomial, packed fp32 operations where the
-// hardware has them (ten issue slots and two MUFU operations an element).
-// h is zero in fp32 beyond |x| = 16, where the limit keeps an infinity out of
-// 0 * inf; a NaN comes through the maximum.
+// max(x, 0), a NaN stays one.
 __device__ __forceinline__ float relu_nan(float x) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(0.f));
   return r;
 }
 
-__device__ __forceinline__ void gelu_erf2(float& x0, float& x1) {
-  const float a0 = fminf(fabsf(x0), 16.f), a1 = fminf(fabsf(x1), 16.f);
-  float d0, d1, t0, t1, p0, p1, g0, g1, e0, e1;
-  constexpr float kP = 0.3275911f * 0.70710678118654752f;
-  constexpr float kQ = 0.84932180028801905f;  // sqrt(log2(e) / 2)
-  fma2v(d0, d1, a0, a1, kP, kP, 1.f, 1.f);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(d0));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(d1));
-  fma2v(p0, p1, t0, t1, -0.5f * 1.061405429f, -0.5f * 1.061405429f, 0.5f * 1.453152027f,
-        0.5f * 1.453152027f);
-  fma2v(p0, p1, p0, p1, t0, t1, -0.5f * 1.421413741f, -0.5f * 1.421413741f);
-  fma2v(p0, p1, p0, p1, t0, t1, 0.5f * 0.284496736f, 0.5f * 0.284496736f);
-  fma2v(p0, p1, p0, p1, t0, t1, -0.5f * 0.254829592f, -0.5f * 0.254829592f);
-  g0 = a0 * kQ;
-  g1 = a1 * kQ;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(-g0 * g0));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(-g1 * g1));
-  // |x| t e first: p is then the only factor of order one left.
-  g0 = a0 * t0 * e0;
-  g1 = a1 * t1 * e1;
-  fma2v(x0, x1, p0, p1, g0, g1, relu_nan(x0), relu_nan(x1));
+// Erf GELU of two values in seven issue slots and one MUFU operation each
+// (gelu_erf in common.cuh: eighteen and two; with one or two warps a
+// sub-partition an activation of 128 values a thread is bound by them):
+//   GELU(x) = max(x, 0) - a Phi(-a), a = |x|,
+// with log2 Phi(-a) by a polynomial of degree seven on [0, 6], fitted by
+// Lawson's iteration (weighted least squares towards the minimax) to the
+// error of a Phi(-a): 2.5e-7 absolute in fp32, and 6e-5 relative in the
+// negative tail.  Beyond 6 the tail stays at its -6e-9.  A NaN comes through
+// the maximum.
+__device__ __forceinline__ void gelu_pair(float& x0, float& x1) {
+  const float a0 = fminf(fabsf(x0), 6.f), a1 = fminf(fabsf(x1), 6.f);
+  float q0, q1, e0, e1;
+  fma2v(q0, q1, a0, a1, -1.43977059e-06f, -1.43977059e-06f, 5.48538883e-05f, 5.48538883e-05f);
+  fma2v(q0, q1, q0, q1, a0, a1, -0.000887982082f, -0.000887982082f);
+  fma2v(q0, q1, q0, q1, a0, a1, 0.00838699006f, 0.00838699006f);
+  fma2v(q0, q1, q0, q1, a0, a1, -0.0538126267f, -0.0538126267f);
+  fma2v(q0, q1, q0, q1, a0, a1, -0.458510876f, -0.458510876f);
+  fma2v(q0, q1, q0, q1, a0, a1, -1.15127623f, -1.15127623f);
+  fma2v(q0, q1, q0, q1, a0, a1, -0.999986351f, -0.999986351f);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(q0));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(q1));
+  fma2v(x0, x1, -a0, -a1, e0, e1, relu_nan(x0), relu_nan(x1));
 }
 
 // Four consecutive elements of a row: raw as loaded (16 or 8 bytes), widened

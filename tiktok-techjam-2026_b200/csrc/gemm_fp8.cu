@@ -42,7 +42,6 @@ struct GemmF8Args {
   int out_dtype, act;
   int splits;  // CTAs per cluster (a power of two)
   int first_tile, end_tile;  // wide kernel: the tiles of this launch
-  bool wide_stores;  // C and its rows start on 32-byte boundaries
 };
 
 template <int BT>
@@ -109,8 +108,8 @@ __device__ __forceinline__ void finish4(const GemmF8Args& args, float4 v, float4
   v.z += bias.z;
   v.w += bias.w;
   if (args.act == 1) {
-    gelu_erf2(v.x, v.y);
-    gelu_erf2(v.z, v.w);
+    gelu_pair(v.x, v.y);
+    gelu_pair(v.z, v.w);
   }
   if (args.out_dtype == TJB_E4M3) {
     if (n >= args.N) v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -432,12 +431,13 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
 //   warp 0        TMA producer
 //   warp 1        MMA issuer: per k-block four K = 32 MMAs into
 //                 one of two 256-column TMEM accumulators
-//   warps 2, 3    products sa[m, kb] sw[n / 128, kb] of the tile's rows, eight
-//                 k-blocks at a time, a ring slot ahead of their use
+//   warps 2, 3    products sa[m, kb] sw[n / 128, kb] of the tile's rows, four
+//                 k-blocks at a time, a ring slot ahead of their use, and its
+//                 bias
 //   warps 4..11   two warp groups, 128 columns each: read P_kb from TMEM in
 //                 16-column pieces, the next in flight while one is added to
-//                 128 fp32 sums in registers; then GELU, rounding, and 32-byte
-//                 stores (a thread holds 128 consecutive values of a row)
+//                 128 fp32 sums in registers; then GELU, rounding, and TMA
+//                 stores from a staging buffer of their own
 // Per k-block and SM the tensor core takes 512 clocks (128 x 256 x 128 at
 // 8192 products a clock), the multiply-adds 280 (packed pairs, two clocks a
 // warp).  What bounds it is the chain MMA -> barrier -> scaling -> barrier ->
@@ -455,15 +455,18 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
 // CTAs' sums through distributed shared memory and adding them in a fixed
 // order.
 struct WideCfg {
-  static constexpr int kStages = 4;
+  static constexpr int kStages = 3;
   static constexpr int kThreads = 384;
   static constexpr uint32_t kABytes = 128 * kF8BK;
   static constexpr uint32_t kBBytes = 256 * kF8BK;
   static constexpr uint32_t kTmemCols = 512;      // two 256-column accumulators
-  static constexpr int kChunk = 8;                // k-blocks of scale products per ring slot
-  static constexpr uint32_t kScaleBytes = 2 * kChunk * 256 * 4;
+  static constexpr int kChunk = 4;                // k-blocks of scale products per ring slot
+  // Two ring slots of kChunk x 256 scale products, and two tiles' bias.
+  static constexpr uint32_t kScaleBytes = 2 * kChunk * 256 * 4 + 2 * 256 * 4;
+  static constexpr uint32_t kOutTile = 32 * 128;  // 32 rows x 128 bytes, 128-byte swizzle
+  static constexpr uint32_t kOutBytes = 8 * 2 * kOutTile;  // two per scaling warp
   static constexpr uint32_t kSmemBytes =
-      1024 + kStages * (kABytes + kBBytes) + kScaleBytes + 256;
+      1024 + kStages * (kABytes + kBBytes) + kOutBytes + kScaleBytes + 256;
 };
 
 template <int kRegs>
@@ -474,22 +477,6 @@ __device__ __forceinline__ void regs_dec() {
 template <int kRegs>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-
-// 32 consecutive bytes of a row of which `cols` elements (per16 to 16 bytes)
-// exist; one 32-byte store where the matrix allows it (a thread holds a row,
-// so narrower stores would write each 32-byte sector twice).
-__device__ __forceinline__ void store32(void* dst, const uint32_t (&w)[8], int cols, int per16,
-                                        bool wide) {
-  if (wide && cols >= 2 * per16) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]),
-                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-    return;
-  }
-  uint4* p = static_cast<uint4*>(dst);
-  if (cols >= per16) p[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  if (cols >= 2 * per16) p[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 // sum[0..15] += s * p[0..15]
@@ -543,7 +530,7 @@ template <bool kSplit>
 __global__ void __launch_bounds__(WideCfg::kThreads, 1)
     gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmA,
                          const __grid_constant__ CUtensorMap tmB,
-                         const GemmF8Args args) {
+                         const __grid_constant__ CUtensorMap tmC, const GemmF8Args args) {
   using Cfg = WideCfg;
   constexpr int kStages = Cfg::kStages, kChunk = Cfg::kChunk;
   constexpr int BN = 256;
@@ -552,8 +539,10 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sA = smem;
   uint8_t* sB = sA + kStages * Cfg::kABytes;
-  float* sScale = reinterpret_cast<float*>(sB + kStages * Cfg::kBBytes);  // [slot][k-block][half][row]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sScale + 2 * kChunk * 256);
+  uint8_t* sOut = sB + kStages * Cfg::kBBytes;                        // [warp][2][kOutTile]
+  float* sScale = reinterpret_cast<float*>(sOut + Cfg::kOutBytes);  // [slot][k-block][row]
+  float* sBias = sScale + 2 * kChunk * 256;                         // [tile & 1][column]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sBias + 2 * 256);
   uint64_t* empty = full + kStages;
   uint64_t* tfull = empty + kStages;
   uint64_t* tempty = tfull + 2;
@@ -583,6 +572,7 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
+    prefetch_tmap(&tmC);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
@@ -672,14 +662,15 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
       umma_commit_w(drain);
       mbar_wait_drain(drain, 0);
     } else if (warp >= 2) {
-      // --------------------------------------------------------- scale products
+      // ------------------------------------------------------- scales and bias
       // Warps 2 and 3 take 64 rows each, two per lane.
       const int num_nb = (args.N + kQBlock - 1) / kQBlock;
       const int r = (warp - 2) * 64 + lane;
       // Row-major scales whose rows start on 16-byte boundaries: four at a time.
       const bool vec = args.as_blk == 1 && args.as_row % 4 == 0 &&
                        (reinterpret_cast<uintptr_t>(args.a_scales) & 15u) == 0;
-      uint32_t c = 0;
+      uint32_t c = 0, odd = 0;
+      float4 bias;
       bool ok = true;
       for (int t = first; ok && t < end; t += step) {
         int m_blk, n_blk;
@@ -692,18 +683,24 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
             args.a_scales + min(row + 32, static_cast<int64_t>(args.M - 1)) * args.as_row;
         const float* w0 = args.w_scales + static_cast<int64_t>(2 * n_blk) * num_k;
         const float* w1 = 2 * n_blk + 1 < num_nb ? w0 + num_k : w0;
+        if constexpr (!kSplit) {
+          // This tile's bias, ready with its first scales (the slot's last
+          // readers are two tiles back, before scales that were waited for).
+          const int n = n_blk * BN + (warp - 2) * 128 + lane * 4;
+          float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (args.bias != nullptr && n < args.N)
+            b = __ldg(reinterpret_cast<const float4*>(args.bias + n));
+          bias = b;
+        }
         for (int kb0 = k0; ok && kb0 < k1; kb0 += kChunk, ++c) {
-          float va[kChunk], vb[kChunk], s0[kChunk], s1[kChunk];
+          float va[kChunk], vb[kChunk];
           if (vec && kb0 % 4 == 0 && kb0 + kChunk <= k1) {
 #pragma unroll
             for (int u = 0; u < kChunk; u += 4) {
-              *reinterpret_cast<float4*>(va + u) = __ldg(reinterpret_cast<const float4*>(a0 + kb0 + u));
-              *reinterpret_cast<float4*>(vb + u) = __ldg(reinterpret_cast<const float4*>(a1 + kb0 + u));
-            }
-#pragma unroll
-            for (int u = 0; u < kChunk; ++u) {
-              s0[u] = __ldg(w0 + kb0 + u);
-              s1[u] = __ldg(w1 + kb0 + u);
+              *reinterpret_cast<float4*>(va + u) =
+                  __ldg(reinterpret_cast<const float4*>(a0 + kb0 + u));
+              *reinterpret_cast<float4*>(vb + u) =
+                  __ldg(reinterpret_cast<const float4*>(a1 + kb0 + u));
             }
           } else {
 #pragma unroll
@@ -711,9 +708,13 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
               const int kb = min(kb0 + u, k1 - 1);
               va[u] = __ldg(a0 + kb * args.as_blk);
               vb[u] = __ldg(a1 + kb * args.as_blk);
-              s0[u] = __ldg(w0 + kb);
-              s1[u] = __ldg(w1 + kb);
             }
+          }
+          float s0[kChunk], s1[kChunk];
+#pragma unroll
+          for (int u = 0; u < kChunk; ++u) {
+            s0[u] = __ldg(w0 + min(kb0 + u, k1 - 1));
+            s1[u] = __ldg(w1 + min(kb0 + u, k1 - 1));
           }
           ok = __all_sync(0xffffffffu,
                           mbar_wait(&sempty[c & 1], ((c >> 1) & 1) ^ 1, abort_flag));
@@ -724,6 +725,10 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
             dst[u * 256 + 32] = vb[u] * s0[u];
             dst[u * 256 + 128] = va[u] * s1[u];
             dst[u * 256 + 160] = vb[u] * s1[u];
+          }
+          if (!kSplit && kb0 == k0) {
+            reinterpret_cast<float4*>(sBias + odd * 256)[(warp - 2) * 32 + lane] = bias;
+            odd ^= 1;
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sfull[c & 1]);
@@ -741,32 +746,37 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
     const int quad = warp & 3;         // TMEM lanes this warp may access
     const int half = (warp - 4) >> 2;  // 128-column half of the tile
     const int r = quad * 32 + lane;    // token row of the tile
+    uint8_t* buf = sOut + (warp - 4) * 2 * Cfg::kOutTile;
     const uint32_t taddr0 =
         tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 128);
     uint32_t it = 0, chunk = 0;  // k-blocks and scale chunks done, over all tiles
+    uint32_t odd = 0;            // tiles done, parity
     bool ok = true;
     bool met = !kSplit;  // this warp has been at the cluster's two meetings
     for (int t = first; ok && t < end; t += step) {
       int m_blk, n_blk;
       coords(t, m_blk, n_blk);
       const int n0 = n_blk * BN + half * 128;
-      // The sums start from the bias; columns past N stay exactly zero (their
-      // weight rows load as zeros), as a ragged 8-bit block's scale needs.
+      // The sums start from the bias, which comes with the first scales;
+      // columns past N stay exactly zero (their weight rows load as zeros), as
+      // a ragged 8-bit block's scale needs.
+      ok = mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag) && ok;
       float sum[128];
 #pragma unroll
       for (int j = 0; j < 128; j += 4) {
         float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!kSplit && args.bias != nullptr && n0 + j < args.N)
-          b = __ldg(reinterpret_cast<const float4*>(args.bias + n0 + j));
+        if (!kSplit) b = reinterpret_cast<const float4*>(sBias + odd * 256 + half * 128)[j / 4];
         sum[j] = b.x;
         sum[j + 1] = b.y;
         sum[j + 2] = b.z;
         sum[j + 3] = b.w;
       }
+      odd ^= 1;
 #pragma unroll 1
       for (int kb = k0; kb < k1; ++kb, ++it) {
         const int u = (kb - k0) & (kChunk - 1);
-        if (u == 0) ok = mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag) && ok;
+        if (u == 0 && kb > k0)
+          ok = mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag) && ok;
         const float s = sScale[((chunk & 1) * kChunk + u) * 256 + half * 128 + r];
         const uint32_t acc = it & 1;
         ok = mbar_wait(&tfull[acc], (it >> 1) & 1, abort_flag) && ok;
@@ -827,49 +837,72 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
       if (n0 >= args.N) continue;  // warp-uniform
       if (args.act == 1) {
 #pragma unroll
-        for (int j = 0; j < 128; j += 2) gelu_erf2(sum[j], sum[j + 1]);
+        for (int j = 0; j < 128; j += 2) gelu_pair(sum[j], sum[j + 1]);
       }
-      const int64_t row = static_cast<int64_t>(m_blk) * 128 + r;
-      if (row >= args.M) continue;
-      const int cols = min(args.N - n0, 128);
+      const int row0 = m_blk * 128 + quad * 32;
+      // Up to two 32-row x 128-byte pieces of this warp at a time: wait until
+      // the stores that last read the buffers are done, write the rows (16-byte
+      // chunk k of row l at k ^ (l & 7)), hand them to TMA.  Stored straight
+      // from registers, a row per lane, the output went out at 16 bytes a clock
+      // (64 KB of fp16: 4100 clocks of a K = 1024 tile's 12000).
+      auto out_free = [&]() {
+        if (lane == 0) bulk_wait_read<0>();
+        __syncwarp();
+      };
+      auto out_send = [&](int pieces, int col, int per_piece) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          for (int c = 0; c < pieces; ++c)
+            if (col + c * per_piece < args.N)
+              tma_store_2d(&tmC, buf + c * Cfg::kOutTile, col + c * per_piece, row0);
+          bulk_commit();
+        }
+      };
+      out_free();
       if (args.out_dtype == TJB_E4M3) {
         float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < 128; ++j) top = max_abs(top, sum[j]);
+        for (int j = 0; j < 128; j += 2) top = max_abs(top, sum[j], sum[j + 1]);
         const float s = block_scale(top);
         const float inv = reciprocal(s);
-        args.c_scales[row * ((args.N + kQBlock - 1) / kQBlock) + n0 / kQBlock] = s;
-        uint8_t* dst = static_cast<uint8_t*>(args.C) + row * args.ldc + n0;
+        uint32_t w[32];
 #pragma unroll
-        for (int j = 0; j < 128; j += 32) {
-          uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = quantize4(&sum[j + 4 * i], s, inv);
-          store32(dst + j, w, cols - j, 16, args.wide_stores);
-        }
+        for (int j = 0; j < 32; ++j) w[j] = quantize4(&sum[4 * j], s, inv);
+        stage_row(buf, lane, w);
+        out_send(1, n0, 128);
+        if (row0 + lane < args.M)
+          args.c_scales[static_cast<int64_t>(row0 + lane) * ((args.N + kQBlock - 1) / kQBlock) +
+                        n0 / kQBlock] = s;
       } else if (args.out_dtype == TJB_F32) {
-        float* dst = static_cast<float*>(args.C) + row * args.ldc + n0;
 #pragma unroll
-        for (int j = 0; j < 128; j += 8) {
-          uint32_t w[8];
+        for (int c = 0; c < 4; ++c) {
+          if (c == 2) {
+            out_send(2, n0, 32);
+            out_free();
+          }
+          uint32_t w[32];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(sum[j + i]);
-          store32(dst + j, w, cols - j, 4, args.wide_stores);
+          for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(sum[c * 32 + j]);
+          stage_row(buf + (c & 1) * Cfg::kOutTile, lane, w);
         }
+        out_send(2, n0 + 64, 32);
       } else {
-        uint16_t* dst = static_cast<uint16_t*>(args.C) + row * args.ldc + n0;
 #pragma unroll
-        for (int j = 0; j < 128; j += 16) {
-          uint32_t w[8];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[32];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = args.out_dtype == TJB_BF16
-                       ? Pack2<__nv_bfloat16>::pack(sum[j + 2 * i], sum[j + 2 * i + 1])
-                       : Pack2<__half>::pack(sum[j + 2 * i], sum[j + 2 * i + 1]);
-          store32(dst + j, w, cols - j, 8, args.wide_stores);
+          for (int j = 0; j < 32; ++j)
+            w[j] = args.out_dtype == TJB_BF16
+                       ? Pack2<__nv_bfloat16>::pack(sum[c * 64 + 2 * j], sum[c * 64 + 2 * j + 1])
+                       : Pack2<__half>::pack(sum[c * 64 + 2 * j], sum[c * 64 + 2 * j + 1]);
+          stage_row(buf + c * Cfg::kOutTile, lane, w);
         }
+        out_send(2, n0, 64);
       }
     }
+    // Every bulk store has completed before the CTA exits.
+    if (lane == 0) bulk_wait_all();
     if (!met) {  // no tile (a live-tile list with fewer): the same meetings
       __syncwarp();
       cluster_sync();
@@ -934,13 +967,15 @@ int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
   using Cfg = WideCfg;
   WideLimits lim;
   if (const int st = wide_limits(lim)) return st;
-  CUtensorMap tmA, tmB;
+  CUtensorMap tmA, tmB, tmC;
   int st = make_tmap_2d(&tmA, TJB_E4M3, A, args.K, args.M, lda, kF8BK, 128);
   if (st != TJB_OK) return st;
   st = make_tmap_2d(&tmB, TJB_E4M3, W, args.K, args.N, ldw, kF8BK, 256);
   if (st != TJB_OK) return st;
-  const int64_t esz = args.out_dtype == TJB_F32 ? 4 : args.out_dtype == TJB_E4M3 ? 1 : 2;
-  args.wide_stores = ((reinterpret_cast<uintptr_t>(args.C) | (args.ldc * esz)) & 31) == 0;
+  const int esz = args.out_dtype == TJB_F32 ? 4 : args.out_dtype == TJB_E4M3 ? 1 : 2;
+  st = make_tmap_2d(&tmC, args.out_dtype, args.C, args.N, args.M,
+                    static_cast<uint64_t>(args.ldc) * esz, 128 / esz, 32);
+  if (st != TJB_OK) return st;
   const int64_t tiles64 =
       (static_cast<int64_t>(args.M) + 127) / 128 * ((args.N + 255) / 256);
   if (tiles64 > 1073741823) return TJB_ERR_BAD_SHAPE;
@@ -961,7 +996,7 @@ int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
     args.splits = 1;
     const int grid = whole < sms ? whole : sms;
     st = launch_kernel(gemm_fp8_wide_kernel<false>, dim3(grid), dim3(Cfg::kThreads),
-                       Cfg::kSmemBytes, stream, tmA, tmB, args);
+                       Cfg::kSmemBytes, stream, tmA, tmB, tmC, args);
     if (st != TJB_OK) return st;
   }
   if (whole < tiles) {
@@ -971,7 +1006,7 @@ int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
     st = launch_kernel_cluster(gemm_fp8_wide_kernel<true>,
                                dim3(static_cast<unsigned>(tiles - whole) << log2),
                                dim3(Cfg::kThreads), Cfg::kSmemBytes, stream,
-                               static_cast<unsigned>(args.splits), tmA, tmB, args);
+                               static_cast<unsigned>(args.splits), tmA, tmB, tmC, args);
   }
   return st;
 }
