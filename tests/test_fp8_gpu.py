@@ -274,7 +274,12 @@ GEMM_SHAPES = [(1, 64, 16), (1, 4096, 4096), (2, 136, 128), (15, 384, 1040), (16
                (17, 1024, 48), (32, 128, 512), (33, 264, 2064), (64, 640, 256), (65, 1160, 144),
                (127, 256, 1024), (128, 128, 128), (129, 120, 640), (300, 1000, 1040),
                (513, 2048, 272), (1000, 768, 768), (2000, 1160, 4096), (2500, 4096, 1024),
-               (5000, 1024, 1040)]
+               (5000, 1024, 1040),
+               # On 148 SMs: wide tiles whose k-blocks are split over clusters
+               # of two, four and eight; rounds of wide tiles with the rows left
+               # over in 64-token tiles, and with the tiles left over split.
+               (1900, 1024, 4096), (1000, 1016, 8192), (600, 512, 16384), (5000, 1024, 4096),
+               (640, 8192, 8192)]
 
 
 @pytest.mark.parametrize("m,n,k", GEMM_SHAPES)
@@ -292,7 +297,7 @@ def test_gemm_fp8(m, n, k, bias, act):
         check_quantised(q, s, ref, tol)
 
 
-@pytest.mark.parametrize("m", [1, 20, 40, 100, 700, 3000])
+@pytest.mark.parametrize("m", [1, 20, 40, 100, 700, 11000])
 def test_gemm_fp8_strides(m):
     """Scales in either order, rows at a pitch, a pitched output whose gaps
     stay as they were."""
@@ -314,7 +319,7 @@ def test_gemm_fp8_strides(m):
     assert torch.equal(whole, out[:, :n])
 
 
-@pytest.mark.parametrize("m", [5, 90, 600, 2600])
+@pytest.mark.parametrize("m", [5, 90, 600, 9000])
 def test_gemm_fp8_bad_values_stay_in_their_rows(m):
     """A NaN or an infinity in one token's operand or scale reaches that
     token's outputs only."""
@@ -354,7 +359,7 @@ def test_gemm_fp8_same_bits_again():
 
 # ------------------------------------------------------------- padded batches
 
-@pytest.mark.parametrize("seq", [200, 1024])
+@pytest.mark.parametrize("seq", [200, 1024, 8192])
 def test_live_tiles(seq):
     """With a live-tile list, rows of unlisted tiles are left as they were and
     the listed ones come out as without it."""
@@ -391,7 +396,7 @@ def test_live_tiles(seq):
     assert torch.equal(out[live], full[live]) and (out[~live] == 3).all()
 
 
-@pytest.mark.parametrize("rows", [1, 100, 700])
+@pytest.mark.parametrize("rows", [1, 100, 700, 70000])
 def test_no_live_tiles(rows):
     g = gen(rows, 9)
     tiles = torch.zeros(1 + (rows + 127) // 128, dtype=torch.int32, device=DEV)

@@ -983,13 +983,13 @@ int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
   const int sms = lim.clusters[0];
   const int num_k = (args.K + kF8BK - 1) / kF8BK;
   // Whole rounds of one tile per SM, then the tiles left over with their
-  // k-blocks split over as many CTAs as run at once.  Splitting costs a second
-  // launch and the exchange, together about 4 k-blocks' time.
+  // k-blocks split over as many CTAs as run at once.  The second launch and
+  // the meeting of the parts take about as long as 26 k-blocks, without a
+  // first launch the meeting about ten.
   int whole = tiles / sms * sms;
   int log2 = 0;
   while (log2 < 3 && 2 << log2 <= num_k && tiles - whole <= lim.clusters[log2 + 1]) ++log2;
-  if (whole < tiles && (log2 == 0 || num_k - (num_k >> log2) < (whole > 0 ? 10 : 4)))
-    whole = tiles;
+  if (whole < tiles && num_k - (num_k >> log2) < (whole > 0 ? 26 : 10)) whole = tiles;
   if (whole > 0) {
     args.first_tile = 0;
     args.end_tile = whole;
@@ -1061,8 +1061,27 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
   // faster than those of a wide tile, but a 64 x 128 tile keeps the tensor
   // core a third as busy (N4096 K4096: M128 10.8 against 15.0 us, M256 16.1 and
   // 16.0, M512 26.7 and 17.8; N1024 K1024: M512 7.2 and 10.9).
-  const int64_t blocks = ((static_cast<int64_t>(M) + 63) / 64) * ((N + 127) / 128) *
-                         ((K + kF8BK - 1) / kF8BK);
-  if (M <= 64 || blocks <= 28 * num_sms()) return launch_skinny<64>(A, W, args, lda, ldw, s);
+  const int num_k = (K + kF8BK - 1) / kF8BK, sms = num_sms();
+  const int64_t num_n = (N + 127) / 128;
+  auto blocks = [&](int64_t m) { return (m + 63) / 64 * num_n * num_k; };
+  if (M <= 64 || blocks(M) <= 28 * sms) return launch_skinny<64>(A, W, args, lda, ldw, s);
+  // Rows that would begin another round of wide tiles go to the 64-token form
+  // where that is sooner done: about 7 us (with its launch) and 2.7 ns a
+  // block, against 0.45 us a k-block and 2.5 us (M5000 N1024 K4096: 36.9 ->
+  // 31.9 us; K1024, where it is not taken: 16.0 against 17.2).
+  const int64_t wide_n = (N + 255) / 256;
+  const int64_t rounds = ((static_cast<int64_t>(M) + 127) / 128 * wide_n + sms - 1) / sms;
+  const int64_t whole = (rounds - 1) * sms / wide_n * 128;  // rows of the other rounds
+  if (rounds > 1 && whole > 0 && m_tiles == nullptr && blocks(M - whole) <= 28 * sms &&
+      7.0 + 0.0027 * blocks(M - whole) < 0.45 * num_k + 2.5) {
+    const int esz = out_dtype == TJB_F32 ? 4 : q ? 1 : 2;
+    args.M = static_cast<int>(whole);
+    if (const int st = launch_wide(A, W, args, lda, ldw, s)) return st;
+    args.M = static_cast<int>(M - whole);
+    args.a_scales += whole * a_scales_row;
+    args.C = static_cast<uint8_t*>(C) + whole * ldc * esz;
+    if (q) args.c_scales += whole * num_n;
+    return launch_skinny<64>(static_cast<const uint8_t*>(A) + whole * lda, W, args, lda, ldw, s);
+  }
   return launch_wide(A, W, args, lda, ldw, s);
 }
