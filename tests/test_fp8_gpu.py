@@ -278,7 +278,7 @@ GEMM_SHAPES = [(1, 64, 16), (1, 4096, 4096), (2, 136, 128), (15, 384, 1040), (16
                # On 148 SMs: wide tiles whose k-blocks are split over clusters
                # of two, four and eight; rounds of wide tiles with the rows left
                # over in 64-token tiles, and with the tiles left over split.
-               (1900, 1024, 4096), (1000, 1016, 8192), (600, 512, 16384), (5000, 1024, 4096),
+               (1900, 1024, 4096), (1000, 1016, 8192), (500, 1024, 16384), (5000, 1024, 4096),
                (640, 8192, 8192)]
 
 

@@ -962,11 +962,11 @@ int wide_limits(WideLimits& lim) {
   return TJB_OK;
 }
 
-int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
-                cudaStream_t stream) {
+// The first `whole` tiles in rounds of one per SM; the others, if any, with
+// their k-blocks split over clusters of 1 << log2 CTAs.
+int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw, int whole,
+                int log2, cudaStream_t stream) {
   using Cfg = WideCfg;
-  WideLimits lim;
-  if (const int st = wide_limits(lim)) return st;
   CUtensorMap tmA, tmB, tmC;
   int st = make_tmap_2d(&tmA, TJB_E4M3, A, args.K, args.M, lda, kF8BK, 128);
   if (st != TJB_OK) return st;
@@ -976,20 +976,8 @@ int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
   st = make_tmap_2d(&tmC, args.out_dtype, args.C, args.N, args.M,
                     static_cast<uint64_t>(args.ldc) * esz, 128 / esz, 32);
   if (st != TJB_OK) return st;
-  const int64_t tiles64 =
-      (static_cast<int64_t>(args.M) + 127) / 128 * ((args.N + 255) / 256);
-  if (tiles64 > 1073741823) return TJB_ERR_BAD_SHAPE;
-  const int tiles = static_cast<int>(tiles64);
-  const int sms = lim.clusters[0];
-  const int num_k = (args.K + kF8BK - 1) / kF8BK;
-  // Whole rounds of one tile per SM, then the tiles left over with their
-  // k-blocks split over as many CTAs as run at once.  The second launch and
-  // the meeting of the parts take about as long as 26 k-blocks, without a
-  // first launch the meeting about ten.
-  int whole = tiles / sms * sms;
-  int log2 = 0;
-  while (log2 < 3 && 2 << log2 <= num_k && tiles - whole <= lim.clusters[log2 + 1]) ++log2;
-  if (whole < tiles && num_k - (num_k >> log2) < (whole > 0 ? 26 : 10)) whole = tiles;
+  const int tiles = (args.M + 127) / 128 * ((args.N + 255) / 256);
+  const int sms = num_sms();
   if (whole > 0) {
     args.first_tile = 0;
     args.end_tile = whole;
@@ -1054,34 +1042,59 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
   args.out_dtype = out_dtype;
   args.act = act;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // The narrowest tile that holds every token.
+  // Up to 64 tokens: the narrowest tile that holds them.
   if (M <= 16) return launch_skinny<16>(A, W, args, lda, ldw, s);
   if (M <= 32) return launch_skinny<32>(A, W, args, lda, ldw, s);
-  // Beyond, the 64-token form while the product is small: its parts meet
-  // faster than those of a wide tile, but a 64 x 128 tile keeps the tensor
-  // core a third as busy (N4096 K4096: M128 10.8 against 15.0 us, M256 16.1 and
-  // 16.0, M512 26.7 and 17.8; N1024 K1024: M512 7.2 and 10.9).
-  const int num_k = (K + kF8BK - 1) / kF8BK, sms = num_sms();
-  const int64_t num_n = (N + 127) / 128;
-  auto blocks = [&](int64_t m) { return (m + 63) / 64 * num_n * num_k; };
-  if (M <= 64 || blocks(M) <= 28 * sms) return launch_skinny<64>(A, W, args, lda, ldw, s);
-  // Rows that would begin another round of wide tiles go to the 64-token form
-  // where that is sooner done: about 7 us (with its launch) and 2.7 ns a
-  // block, against 0.45 us a k-block and 2.5 us (M5000 N1024 K4096: 36.9 ->
-  // 31.9 us; K1024, where it is not taken: 16.0 against 17.2).
-  const int64_t wide_n = (N + 255) / 256;
-  const int64_t rounds = ((static_cast<int64_t>(M) + 127) / 128 * wide_n + sms - 1) / sms;
-  const int64_t whole = (rounds - 1) * sms / wide_n * 128;  // rows of the other rounds
-  if (rounds > 1 && whole > 0 && m_tiles == nullptr && blocks(M - whole) <= 28 * sms &&
-      7.0 + 0.0027 * blocks(M - whole) < 0.45 * num_k + 2.5) {
-    const int esz = out_dtype == TJB_F32 ? 4 : q ? 1 : 2;
-    args.M = static_cast<int>(whole);
-    if (const int st = launch_wide(A, W, args, lda, ldw, s)) return st;
-    args.M = static_cast<int>(M - whole);
-    args.a_scales += whole * a_scales_row;
-    args.C = static_cast<uint8_t*>(C) + whole * ldc * esz;
-    if (q) args.c_scales += whole * num_n;
-    return launch_skinny<64>(static_cast<const uint8_t*>(A) + whole * lda, W, args, lda, ldw, s);
+  if (M <= 64) return launch_skinny<64>(A, W, args, lda, ldw, s);
+  // More: 64-token tiles (quick to start, their parts quick to meet, but the
+  // tensor core a third as busy) or wide ones (in rounds of one per SM, or
+  // split over clusters, or both), by the time that each is expected to take.
+  // The constants, in us, were fitted to 60 shapes of M 65-8000, N 128-8192, K
+  // 128-8192 on a B200 (mean error 7-9 %); the choice comes within 1 % of the
+  // best of the forms on average, 28 % at worst.
+  WideLimits lim;
+  if (const int st = wide_limits(lim)) return st;
+  const int sms = lim.clusters[0];
+  const int num_k = (K + kF8BK - 1) / kF8BK;
+  const int64_t num_n = (N + 127) / 128, wide_n = (N + 255) / 256;
+  const int64_t tiles = (static_cast<int64_t>(M) + 127) / 128 * wide_n;
+  if (tiles > 1073741823) return TJB_ERR_BAD_SHAPE;
+  auto skinny_us = [&](int64_t m) {
+    const double t = static_cast<double>((m + 63) / 64 * num_n);
+    return 4.3 + t * (0.0157 + 0.0024 * num_k);
+  };
+  auto wide_us = [&](int64_t rounds) { return 2.9 + rounds * (0.53 * num_k + 1.75); };
+  const int64_t rounds = (tiles + sms - 1) / sms;
+  double best = skinny_us(M);
+  enum { kSkinny, kWide, kRows } form = kSkinny;
+  int whole = static_cast<int>(tiles), log2 = 0;
+  if (wide_us(rounds) < best) {
+    best = wide_us(rounds);
+    form = kWide;
   }
-  return launch_wide(A, W, args, lda, ldw, s);
+  // The last, partial round: split, or its rows in 64-token tiles.
+  const int64_t full = (rounds - 1) * sms;
+  const double full_us = rounds > 1 ? wide_us(rounds - 1) : 0.0;
+  for (int i = 1; i < 4 && 1 << i <= num_k && tiles - full <= lim.clusters[i]; ++i) {
+    const double us = full_us + 8.9 + 0.66 * num_k / (1 << i);
+    if (us < best) {
+      best = us;
+      form = kWide;
+      whole = static_cast<int>(full);
+      log2 = i;
+    }
+  }
+  const int64_t rows = full / wide_n * 128;  // (a live-tile list is not cut)
+  if (rows > 0 && m_tiles == nullptr && full_us + 1.5 + skinny_us(M - rows) < best) form = kRows;
+  if (form == kSkinny) return launch_skinny<64>(A, W, args, lda, ldw, s);
+  if (form == kWide) return launch_wide(A, W, args, lda, ldw, whole, log2, s);
+  const int esz = out_dtype == TJB_F32 ? 4 : q ? 1 : 2;
+  args.M = static_cast<int>(rows);
+  whole = static_cast<int>(rows / 128 * wide_n);
+  if (const int st = launch_wide(A, W, args, lda, ldw, whole, 0, s)) return st;
+  args.M = static_cast<int>(M - rows);
+  args.a_scales += rows * a_scales_row;
+  args.C = static_cast<uint8_t*>(C) + rows * ldc * esz;
+  if (q) args.c_scales += rows * num_n;
+  return launch_skinny<64>(static_cast<const uint8_t*>(A) + rows * lda, W, args, lda, ldw, s);
 }
