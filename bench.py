@@ -58,6 +58,10 @@ ncu captures are taken with):
     --kernel ffn T D F            (two launches)
     --kernel ffn_single T D F     (one kernel, hidden on chip; d <= 1024)
     --kernel gemm_ln M N K
+    --kernel rms ROWS D           (fp32 residual, fp16 delta, e4m3 output)
+    --kernel quant ROWS K         (fp16 to e4m3, 1 x 128 blocks)
+    --kernel quant_weights N K    (fp16 to e4m3, 128 x 128 blocks)
+    --kernel gemm_fp8 M N K [--act gelu] [--out f16|f32|e4m3]
 """
 
 from __future__ import annotations
@@ -709,10 +713,10 @@ def kernel_main(argv) -> int:
 
     ap = argparse.ArgumentParser(prog="bench.py --kernel")
     ap.add_argument("kernel", choices=["gemm", "attn", "ln", "ffn", "ffn_single", "gemm_ln",
-                                       "small"])
+                                       "small", "rms", "quant", "quant_weights", "gemm_fp8"])
     ap.add_argument("dims", type=int, nargs="+")
     ap.add_argument("--act", choices=["none", "gelu"], default="none")
-    ap.add_argument("--out", choices=["f16", "f32"], default="f16")
+    ap.add_argument("--out", choices=["f16", "f32", "e4m3"], default="f16")
     ap.add_argument("--lengths", choices=["full", "prefix"], default="full")
     ap.add_argument("--stream-k", action="store_true", help="gemm: pass a stream-K workspace")
     ap.add_argument("--launches", type=int, default=5)
@@ -729,6 +733,8 @@ def kernel_main(argv) -> int:
         m, n, k = args.dims
         a, w = randn(m, k), randn(n, k, scale=k ** -0.5)
         bias = torch.randn(n, device=dev, generator=g)
+        if args.out == "e4m3":
+            ap.error("gemm writes f16 or f32")
         out_dtype = torch.float16 if args.out == "f16" else torch.float32
         act = K.ACT_GELU if args.act == "gelu" else K.ACT_NONE
         ws = K.gemm_workspace(dev) if args.stream_k else None
@@ -772,6 +778,30 @@ def kernel_main(argv) -> int:
         fn = lambda: K.gemm_add_layernorm(a, w, bias, res, gamma, beta, 1e-5,
                                           residual_out=res, out=out, workspace=ws)
         flops = 2.0 * m * n * k
+    elif args.kernel == "rms":
+        rows, d = args.dims
+        res = torch.randn(rows, d, device=dev, generator=g)
+        delta = randn(rows, d)
+        w = torch.ones(d, device=dev)
+        fn = lambda: K.fused_add_rmsnorm(res, delta, w, 1e-5, out_dtype=torch.float8_e4m3fn,
+                                         residual_out=res)
+        flops, nbytes = 0.0, rows * d * (4.0 + 2 + 4 + 1)
+    elif args.kernel in ("quant", "quant_weights"):
+        x = randn(*args.dims)
+        fn = (lambda: K.quantize_blocks(x)) if args.kernel == "quant" else \
+            (lambda: K.quantize_weight_blocks(x))
+        flops, nbytes = 0.0, x.numel() * 3.0
+    elif args.kernel == "gemm_fp8":
+        m, n, k = args.dims
+        a, a_scales = K.quantize_blocks(randn(m, k))
+        w, w_scales = K.quantize_weight_blocks(randn(n, k, scale=k ** -0.5))
+        bias = torch.randn(n, device=dev, generator=g)
+        out_dtype = {"f16": torch.float16, "f32": torch.float32,
+                     "e4m3": torch.float8_e4m3fn}[args.out]
+        act = K.ACT_GELU if args.act == "gelu" else K.ACT_NONE
+        fn = lambda: K.gemm_fp8(a, a_scales, w, w_scales, bias, act=act, out_dtype=out_dtype)
+        flops = 2.0 * m * n * k
+        nbytes = float(m * k + n * k + m * n * out_dtype.itemsize)
     elif args.kernel == "small":
         # The whole forward in one launch (tjb_forward_small): dims B S d H F L,
         # default-like random weights, all tokens valid, causal.
