@@ -148,8 +148,8 @@ def rms_ref(res, delta, w, eps):
 
 
 # fp32 error of the norm, relative to the result: the sum of squares goes
-# through at most 32 additions a thread, 5 in the warp and 16 across warps
-# after one rounding of each x (twice in its square) and of each square, so its
+# through at most 53 additions (32 a thread, 5 in the warp and 16 across warps;
+# or 16, 5 and 32) after one rounding of each x (twice in its square) and of each square, so its
 # relative error is below 56 u and the root's half of that; x, 1/sqrt, the two
 # products and the mean's division and sum with eps add at most 6 u.
 NORM_REL = 40 * U32
@@ -205,10 +205,31 @@ def test_add_rmsnorm_odd_width(d):
     check_out(out, ref, NORM_REL * ref.abs())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,offset", [(4, 0), (1000, 0), (1004, 0), (1024, 4), (256, 12)])
+def test_add_rmsnorm_16_bit_odd_rows(d, offset, dtype):
+    """Widths that are no multiple of 16 columns, and rows that start between
+    16-byte borders."""
+    g = gen(d, offset)
+
+    def shifted():
+        return rand(g, 23 * d + 16).to(dtype)[offset:offset + 23 * d].view(23, d)
+
+    for res, delta in ((shifted(), shifted()), (shifted(), rand(g, 23, d).to(dtype)),
+                       (rand(g, 23, d).to(dtype), shifted()), (shifted(), None)):
+        w = rand(g, d)
+        _, ref = rms_ref(res, delta, w, 1e-5)
+        new, out = K().fused_add_rmsnorm(res, delta, w, 1e-5, out_dtype=dtype)
+        check_out(out, ref, NORM_REL * ref.abs())
+        if delta is not None:
+            assert torch.equal(new, (res.float() + delta.float()).to(dtype))
+
+
 @pytest.mark.parametrize("rows,d", [(300, 1024), (7000, 256), (130, 4096)])
-def test_add_rmsnorm_masked_rows_in_place(rows, d):
+@pytest.mark.parametrize("delta_dtype", [torch.float16, torch.bfloat16])
+def test_add_rmsnorm_masked_rows_in_place(rows, d, delta_dtype):
     g = gen(rows, d, 1)
-    res, delta, w = rand(g, rows, d).bfloat16(), rand(g, rows, d).half(), rand(g, d)
+    res, delta, w = rand(g, rows, d).bfloat16(), rand(g, rows, d).to(delta_dtype), rand(g, d)
     mask = torch.rand(rows, device=DEV, generator=g) > 0.4
     _, ref = rms_ref(res, delta, w, 1e-5)
     want = (res.float() + delta.float()).bfloat16()
@@ -360,7 +381,8 @@ def test_gemm_fp8_same_bits_again():
 # ------------------------------------------------------------- padded batches
 
 @pytest.mark.parametrize("seq", [200, 1024, 8192])
-def test_live_tiles(seq):
+@pytest.mark.parametrize("res_dtype", [torch.float32, torch.float16])
+def test_live_tiles(seq, res_dtype):
     """With a live-tile list, rows of unlisted tiles are left as they were and
     the listed ones come out as without it."""
     g = gen(seq)
@@ -373,7 +395,7 @@ def test_live_tiles(seq):
     for t in listed:
         live[t * 128:(t + 1) * 128] = True
     assert live.any() and not live.all()
-    res, delta, w = rand(g, rows, d), rand(g, rows, d).half(), rand(g, d)
+    res, delta, w = rand(g, rows, d).to(res_dtype), rand(g, rows, d).half(), rand(g, d)
     full_res, (fq, fs) = K().fused_add_rmsnorm(res, delta, w, 1e-5, out_dtype=F8)
     keep = res.clone()
     new, (q, s) = K().fused_add_rmsnorm(res, delta, w, 1e-5, out_dtype=F8, residual_out=res,

@@ -170,6 +170,50 @@ __device__ __forceinline__ float4 widen4(const Raw4<k16>& r, bool bf16) {
   }
 }
 
+// Sixteen bytes of a row (four fp32 or eight 16-bit elements) as loaded, with
+// their largest magnitude and their fp32 values.
+template <typename T>
+struct Piece16;
+template <>
+struct Piece16<float> {
+  static constexpr int kElems = 4;
+  float4 v;
+  __device__ __forceinline__ float max_abs() const { return max_abs4(v); }
+  __device__ __forceinline__ void widen(float (&f)[4]) const {
+    f[0] = v.x;
+    f[1] = v.y;
+    f[2] = v.z;
+    f[3] = v.w;
+  }
+};
+template <typename T, typename T2>
+struct Piece16Half {
+  static constexpr int kElems = 8;
+  T2 v[4];
+  __device__ __forceinline__ float max_abs() const {
+    const T2 m = __hmax2_nan(__hmax2_nan(__habs2(v[0]), __habs2(v[1])),
+                             __hmax2_nan(__habs2(v[2]), __habs2(v[3])));
+    return tjb::max_abs(static_cast<float>(m.x), static_cast<float>(m.y));
+  }
+  __device__ __forceinline__ void widen(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = static_cast<float>(v[i].x);
+      f[2 * i + 1] = static_cast<float>(v[i].y);
+    }
+  }
+};
+template <>
+struct Piece16<__half> : Piece16Half<__half, __half2> {};
+template <>
+struct Piece16<__nv_bfloat16> : Piece16Half<__nv_bfloat16, __nv_bfloat162> {};
+
+template <typename T>
+__device__ __forceinline__ Piece16<T> load_piece16(const T* p) {
+  const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(p));
+  return *reinterpret_cast<const Piece16<T>*>(&raw);
+}
+
 // Four consecutive fp32 values rounded once to `dtype` (f32, f16, bf16).
 __device__ __forceinline__ void store4(void* out, int dtype, int64_t idx, float4 y) {
   if (dtype == TJB_F32) {
@@ -185,6 +229,24 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t idx, float4
     raw.y = Pack2<__half>::pack(y.z, y.w);
   }
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + idx) = raw;
+}
+
+// Eight consecutive fp32 values rounded once to `dtype` (16-byte stores).
+__device__ __forceinline__ void store8(void* out, int dtype, int64_t idx, const float (&y)[8]) {
+  if (dtype == TJB_F32) {
+    float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + idx);
+    p[0] = make_float4(y[0], y[1], y[2], y[3]);
+    p[1] = make_float4(y[4], y[5], y[6], y[7]);
+    return;
+  }
+  uint4 raw;
+  if (dtype == TJB_BF16)
+    raw = make_uint4(Pack2<__nv_bfloat16>::pack(y[0], y[1]), Pack2<__nv_bfloat16>::pack(y[2], y[3]),
+                     Pack2<__nv_bfloat16>::pack(y[4], y[5]), Pack2<__nv_bfloat16>::pack(y[6], y[7]));
+  else
+    raw = make_uint4(Pack2<__half>::pack(y[0], y[1]), Pack2<__half>::pack(y[2], y[3]),
+                     Pack2<__half>::pack(y[4], y[5]), Pack2<__half>::pack(y[6], y[7]));
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + idx) = raw;
 }
 
 // Instruction descriptor of kind::f8f6f4 with e4m3 operands (format 0), fp32

@@ -9,50 +9,6 @@ namespace tjb {
 namespace {
 
 constexpr int kQuantThreads = 256;
-// Sixteen bytes of a row (four fp32 or eight 16-bit elements) as loaded, with
-// their largest magnitude and their fp32 values.
-template <typename T>
-struct Piece16;
-template <>
-struct Piece16<float> {
-  static constexpr int kElems = 4;
-  float4 v;
-  __device__ __forceinline__ float max_abs() const { return max_abs4(v); }
-  __device__ __forceinline__ void widen(float (&f)[4]) const {
-    f[0] = v.x;
-    f[1] = v.y;
-    f[2] = v.z;
-    f[3] = v.w;
-  }
-};
-template <typename T, typename T2>
-struct Piece16Half {
-  static constexpr int kElems = 8;
-  T2 v[4];
-  __device__ __forceinline__ float max_abs() const {
-    const T2 m = __hmax2_nan(__hmax2_nan(__habs2(v[0]), __habs2(v[1])),
-                             __hmax2_nan(__habs2(v[2]), __habs2(v[3])));
-    return tjb::max_abs(static_cast<float>(m.x), static_cast<float>(m.y));
-  }
-  __device__ __forceinline__ void widen(float (&f)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = static_cast<float>(v[i].x);
-      f[2 * i + 1] = static_cast<float>(v[i].y);
-    }
-  }
-};
-template <>
-struct Piece16<__half> : Piece16Half<__half, __half2> {};
-template <>
-struct Piece16<__nv_bfloat16> : Piece16Half<__nv_bfloat16, __nv_bfloat162> {};
-
-template <typename T>
-__device__ __forceinline__ Piece16<T> load_piece16(const T* p) {
-  const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(p));
-  return *reinterpret_cast<const Piece16<T>*>(&raw);
-}
-
 // Activations: a warp takes kSteps x 512 bytes of a row, all in flight at
 // once; 32 (fp32) or 16 (16-bit) neighbouring lanes hold one block, so its
 // amax is a few shuffles of values in registers.  Consecutive warps take

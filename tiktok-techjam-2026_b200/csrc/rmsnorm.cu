@@ -5,10 +5,13 @@
 // the unrounded fp32 sum.  The output is f32 / f16 / bf16, or e4m3 with one
 // scale for each row and 128 columns.
 //
-// One row is owned by TPR threads, chunk i of thread t covering columns
-// 4 (i TPR + t) .. +3: the 32 lanes of a warp hold 128 consecutive, aligned
-// columns of a chunk, which is exactly one scale block, so its amax is one
-// warp-wide integer maximum of values already in registers.
+// One row is owned by TPR threads that hold up to four chunks of it in
+// registers, from one read.  Two kernels: 16-byte accesses of eight columns
+// where the residual is 16-bit, the delta absent or of its type and all
+// pointers are 16-byte aligned, and chunks of four columns for every other
+// case.  Consecutive threads take consecutive chunks, so a scale block of 128
+// columns is half a warp or a warp, and its amax an integer maximum of values
+// already in registers.
 #include <type_traits>
 
 #include "fp8.cuh"
@@ -16,12 +19,12 @@
 namespace tjb {
 namespace {
 
-// Row chunks a thread holds (d <= 16 TPR).  Four keep a thread at about 40
-// registers: what counts is the bytes that all threads of an SM have in
-// flight, and eight chunks, weights fetched ahead of the sum, or a persistent
-// block with the next row in flight all lost more by the threads they cost
-// (16384 x 4096, bf16 inputs, 8-bit output: 87 us; 117 with early weights, 124
-// persistent; 65536 x 4096 fp32 + fp16: 432, 436 and 610 us).
+// Row chunks a thread holds (d <= 16 TPR, or 32 TPR with eight columns).  Four
+// keep a thread at 40 to 64 registers: what counts is the bytes that all
+// threads of an SM have in flight.  Eight chunks of four columns, weights
+// fetched ahead of the sum, or a persistent block with the next row in flight
+// lost more by the threads they cost (65536 x 4096, fp32 + fp16 to 8 bits:
+// 432 us, 436 and 610).
 constexpr int kRmsChunks = 4;
 
 // Sum over the TPR threads of a row; every thread of the block calls it.
@@ -125,6 +128,98 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
   }
 }
 
+// The same on 16-byte pieces of eight columns, sixteen lanes to a scale block.
+// 16384 x 4096, bf16 + bf16 to 8 bits: 75 us (floor 72) against 85 in pieces of
+// four, and 79 with two chunks a thread; 8192 x 8192, bf16 alone: 51 against 69.
+template <typename T, bool kDelta, int TPR>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+    add_rmsnorm16_kernel(const T* res, const T* delta, T* res_out, void* out,
+                         float* __restrict__ out_scales, const float* __restrict__ w, int rows,
+                         int d, float eps, int out_dtype, const uint8_t* __restrict__ row_mask,
+                         const int32_t* __restrict__ m_tiles) {
+  constexpr int BLOCK = TPR < 256 ? 256 : TPR;
+  constexpr int kRowsPerBlock = BLOCK / TPR;
+  constexpr int res_dtype = std::is_same<T, __half>::value ? TJB_F16 : TJB_BF16;
+  __shared__ float scratch[BLOCK / 32];
+  const int t = threadIdx.x % TPR;
+  griddep_wait();
+  griddep_launch_dependents();
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + threadIdx.x / TPR;
+  if (m_tiles != nullptr) {
+    const int64_t li = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock / kLiveTileRows;
+    if (li >= __ldg(m_tiles)) return;
+    row = static_cast<int64_t>(__ldg(m_tiles + 1 + li)) * kLiveTileRows + row % kLiveTileRows;
+  }
+  const bool active = row < rows;
+  const int64_t base = row * d;
+  Piece16<T> rr[kRmsChunks], rd[kDelta ? kRmsChunks : 1];
+#pragma unroll
+  for (int i = 0; i < kRmsChunks; ++i) {
+    const int col = (i * TPR + t) * 8;
+    if (active && col < d) {
+      rr[i] = load_piece16(res + base + col);
+      if constexpr (kDelta) rd[i] = load_piece16(delta + base + col);
+    }
+  }
+  float v[kRmsChunks][8];
+  float sq = 0.f;
+#pragma unroll
+  for (int i = 0; i < kRmsChunks; ++i) {
+    const int col = (i * TPR + t) * 8;
+    if (active && col < d) {
+      rr[i].widen(v[i]);
+      if constexpr (kDelta) {
+        float dl[8];
+        rd[i].widen(dl);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] += dl[j];
+      }
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) part += v[i][j] * v[i][j] + v[i][j + 1] * v[i][j + 1];
+      sq += part;
+    }
+  }
+  const float mean = rms_row_sum<TPR>(sq, scratch) / static_cast<float>(d);
+  const float rstd = __frsqrt_rn(mean + eps);
+  if (!active) return;  // uniform over each warp
+  const bool keep = row_mask == nullptr || __ldg(row_mask + row) != 0;
+  const int kb_count = (d + kQBlock - 1) / kQBlock;
+#pragma unroll
+  for (int i = 0; i < kRmsChunks; ++i) {
+    const int col = (i * TPR + t) * 8;
+    if (col - (t & 31) * 8 >= d) break;  // warp-uniform
+    float y[8] = {};
+    if (col < d) {
+      if (kDelta && res_out != nullptr) store8(res_out, res_dtype, base + col, v[i]);
+      if (keep) {
+        const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + col));
+        const float4 w1 = __ldg(reinterpret_cast<const float4*>(w + col) + 1);
+        const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = v[i][j] * rstd * ww[j];
+      }
+    }
+    if (out_dtype == TJB_E4M3) {
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) top = max_abs(top, y[j], y[j + 1]);
+      uint32_t bits = abs_bits(top);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+      const float s = block_scale(__uint_as_float(bits));
+      const float inv = reciprocal(s);
+      if (col < d) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(out) + base + col) =
+            make_uint2(quantize4(y, s, inv), quantize4(y + 4, s, inv));
+        if ((t & 15) == 0) out_scales[row * kb_count + col / kQBlock] = s;
+      }
+    } else if (col < d) {
+      store8(out, out_dtype, base + col, y);
+    }
+  }
+}
+
 }  // namespace
 }  // namespace tjb
 
@@ -153,34 +248,62 @@ extern "C" int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out
   if (!device_ok()) return TJB_ERR_NO_DEVICE;
   if (rows == 0) return TJB_OK;
   const int64_t n = m_tiles ? (rows + kLiveTileRows - 1) / kLiveTileRows * kLiveTileRows : rows;
-  // Threads per row: enough for the row (16 columns each); with few rows, up
-  // to one chunk of four columns each, since then the latency of a row counts
-  // and not the number of threads.
+  // 16-byte accesses where the types and the alignment allow them.
+  const bool vec8 = res_dtype != TJB_F32 && (!delta || delta_dtype == res_dtype) && d % 8 == 0 &&
+                    aligned16(res) && (!delta || aligned16(delta)) &&
+                    (!res_out || aligned16(res_out)) && aligned16(out);
+  // Threads per row: enough for the row; with few rows, up to one chunk each,
+  // since then the latency of a row counts and not the number of threads.
+  const int chunk = vec8 ? 8 : 4;
   int tpr = 32;
-  while (16 * tpr < d || (tpr < 1024 && 4 * tpr < d && 2 * n * tpr <= 1024 * num_sms())) tpr *= 2;
-  auto go = [&](auto tprc, auto res16, auto kdelta) {
-    constexpr int TPR = decltype(tprc)::value;
-    constexpr int block = TPR < 256 ? 256 : TPR, per_block = block / TPR;
-    return launch_kernel(add_rmsnorm_kernel<TPR, decltype(res16)::value, decltype(kdelta)::value>,
-                         dim3(static_cast<unsigned>((n + per_block - 1) / per_block)), dim3(block),
-                         0, reinterpret_cast<cudaStream_t>(stream), res, delta, res_out, out,
-                         out_scales, w, static_cast<int>(rows), d, eps, res_dtype, delta_dtype,
-                         out_dtype, row_mask, m_tiles);
-  };
-  auto pick = [&](auto res16, auto kdelta) {
+  while (chunk * kRmsChunks * tpr < d ||
+         (tpr < 1024 && chunk * tpr < d && 2 * n * tpr <= 1024 * num_sms()))
+    tpr *= 2;
+  auto by_tpr = [&](auto run) {
     switch (tpr) {
-      case 32: return go(std::integral_constant<int, 32>{}, res16, kdelta);
-      case 64: return go(std::integral_constant<int, 64>{}, res16, kdelta);
-      case 128: return go(std::integral_constant<int, 128>{}, res16, kdelta);
-      case 256: return go(std::integral_constant<int, 256>{}, res16, kdelta);
-      case 512: return go(std::integral_constant<int, 512>{}, res16, kdelta);
-      default: return go(std::integral_constant<int, 1024>{}, res16, kdelta);
+      case 32: return run(std::integral_constant<int, 32>{});
+      case 64: return run(std::integral_constant<int, 64>{});
+      case 128: return run(std::integral_constant<int, 128>{});
+      case 256: return run(std::integral_constant<int, 256>{});
+      case 512: return run(std::integral_constant<int, 512>{});
+      default: return run(std::integral_constant<int, 1024>{});
     }
   };
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  auto grid = [&](int per_block) {
+    return dim3(static_cast<unsigned>((n + per_block - 1) / per_block));
+  };
+  if (vec8) {
+    auto go = [&](auto type, auto kdelta) {
+      using T = decltype(type);
+      constexpr bool kDelta = decltype(kdelta)::value;
+      return by_tpr([&](auto tprc) {
+        constexpr int TPR = decltype(tprc)::value;
+        constexpr int block = TPR < 256 ? 256 : TPR;
+        return launch_kernel(add_rmsnorm16_kernel<T, kDelta, TPR>, grid(block / TPR), dim3(block),
+                             0, st, static_cast<const T*>(res), static_cast<const T*>(delta),
+                             static_cast<T*>(res_out), out, out_scales, w, static_cast<int>(rows),
+                             d, eps, out_dtype, row_mask, m_tiles);
+      });
+    };
+    if (res_dtype == TJB_F16)
+      return delta ? go(__half{}, std::true_type{}) : go(__half{}, std::false_type{});
+    return delta ? go(__nv_bfloat16{}, std::true_type{}) : go(__nv_bfloat16{}, std::false_type{});
+  }
+  auto go = [&](auto res16, auto kdelta) {
+    return by_tpr([&](auto tprc) {
+      constexpr int TPR = decltype(tprc)::value;
+      constexpr int block = TPR < 256 ? 256 : TPR;
+      return launch_kernel(
+          add_rmsnorm_kernel<TPR, decltype(res16)::value, decltype(kdelta)::value>,
+          grid(block / TPR), dim3(block), 0, st, res, delta, res_out, out, out_scales, w,
+          static_cast<int>(rows), d, eps, res_dtype, delta_dtype, out_dtype, row_mask, m_tiles);
+    });
+  };
   auto with_delta = [&](auto res16) {
-    if (!delta) return pick(res16, std::integral_constant<int, 0>{});
-    if (delta_dtype == TJB_F32) return pick(res16, std::integral_constant<int, 1>{});
-    return pick(res16, std::integral_constant<int, 2>{});
+    if (!delta) return go(res16, std::integral_constant<int, 0>{});
+    if (delta_dtype == TJB_F32) return go(res16, std::integral_constant<int, 1>{});
+    return go(res16, std::integral_constant<int, 2>{});
   };
   return res_dtype == TJB_F32 ? with_delta(std::false_type{}) : with_delta(std::true_type{});
 }
