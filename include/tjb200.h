@@ -397,7 +397,8 @@ int tjb_forward_small(const tjb_small_layer* layers, int L, const float* lnf_w,
  *
  * tjb_quantize_blocks: x [rows, K] (in_dtype f32, f16 or bf16; rows ldx
  * elements apart) -> q [rows, K] e4m3 and scales [rows, ceil(K/128)], both
- * contiguous.  K % 16 == 0; x, its rows and q start on 16-byte boundaries.
+ * contiguous.  K % 16 == 0, K <= 2^31 - 1025; x, its rows and q start on
+ * 16-byte boundaries.
  * m_tiles (nullable) as in tjb_row_tiles: rows of unlisted tiles
  * are neither read nor written.
  * tjb_quantize_weight_blocks: w [N, K] (rows ldw elements apart) ->
@@ -437,9 +438,11 @@ int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out, void* out
  * bytes apart) with w_scales contiguous [ceil(N/128), ceil(K/128)]; bias fp32
  * [N] or NULL; act: 0 = none, 1 = exact erf GELU.  C (rows ldc elements
  * apart): f32, f16, bf16, or TJB_E4M3 with c_scales contiguous
- * [M, ceil(N/128)].  fp32 accumulation; a call's result depends on nothing
- * but its operands (no atomics, no workspace).  K % 16 == 0, N % 8 == 0
- * (e4m3 output: N % 16 == 0), lda and ldw multiples of 16, ldc of 8 (e4m3:
+ * [M, ceil(N/128)].  fp32 accumulation; sa * sw is one fp32 product, so
+ * scales whose product leaves the type's normal range lose what it cannot
+ * hold.  A call's result depends on nothing but its operands (no atomics, no
+ * workspace).  K % 16 == 0, N % 8 == 0 (e4m3 output: N % 16 == 0), both at
+ * most 2^31 - 1025; lda and ldw multiples of 16, ldc of 8 (e4m3:
  * 16); 16-byte aligned A, W, C and bias.  m_tiles (nullable) as in
  * tjb_row_tiles.
  * The 8-bit sibling of tjb_gemm_bias; no counterpart in the reference.

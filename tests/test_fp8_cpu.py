@@ -28,6 +28,7 @@ def test_quantize_refusals(fn):
     assert quantize(fn=fn, k=24) == 2
     assert quantize(fn=fn, ldx=128) == 2
     assert quantize(fn=fn, rows=2 ** 31) == 2
+    assert quantize(fn=fn, k=2 ** 31 - 16, ldx=2 ** 31 - 16) == 2
     assert quantize(fn=fn, ldx=258) == 3
     assert quantize(fn=fn, x=FAKE + 8) == 3
     assert quantize(fn=fn, x=FAKE + 4, dtype=1) == 3
@@ -81,6 +82,9 @@ def test_gemm_fp8_refusals():
     assert gemm(lda=128) == 2
     assert gemm(ldw=128) == 2
     assert gemm(ldc=128) == 2
+    assert gemm(k=2 ** 31 - 16) == 2         # rounded up, these would pass 2^31
+    assert gemm(n=2 ** 31 - 16) == 2
+    assert gemm(m=2 ** 31 - 1) == 2
     assert gemm(lda=264) == 3
     assert gemm(ldw=264) == 3
     assert gemm(ldc=260, out=1) == 3

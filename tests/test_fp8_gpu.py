@@ -5,6 +5,9 @@ Tolerances count roundings: half a step of the output type, plus the fp32
 error of what is computed before it (derived beside each bound)."""
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -510,6 +513,91 @@ def test_large_offsets():
     ref, tol = product_ref(q[-300:], s[-300:], wq, ws)
     check_out(out[-300:], ref, tol)
     assert (out[:1000] == 0).all()
+
+
+def test_row_pitch_past_32_bits():
+    """Rows of an operand 2^32 + 256 elements apart."""
+    g = gen(2)
+    pitch = (1 << 32) + 256
+    a, sa, w, sw = operands(g, 2, 64, 16)
+    raw = torch.zeros(pitch + 512, dtype=torch.uint8, device=DEV)
+    far = raw.as_strided((2, 16), (pitch, 1)).view(F8)
+    far.view(torch.uint8).copy_(a.view(torch.uint8))
+    raw[256:272] = 0x38
+    assert far.stride(0) == pitch
+    assert torch.equal(K().gemm_fp8(far, sa, w, sw), K().gemm_fp8(a, sa, w, sw))
+    out = raw.view(torch.bfloat16).as_strided((2, 64), (1 << 31, 1))
+    with pytest.raises(ValueError):
+        K().gemm_fp8(a, sa, w, sw, out=out)
+    half = raw.view(torch.float16)
+    assert half.numel() > 1 << 31
+    with pytest.raises(ValueError):
+        K().quantize_blocks(half[:1 << 31].view(1, -1))
+    with pytest.raises(ValueError):
+        K().quantize_weight_blocks(half[:1 << 31].view(1, -1))
+    many = (1 << 32) + 5
+    with pytest.raises(ValueError):
+        K().gemm_fp8(a[:1].expand(many, 16), sa[:1].expand(many, 1), w, sw)
+
+
+def test_two_streams():
+    """Calls of every form in flight on two streams at once give what each
+    gives alone."""
+    g = gen(12)
+    n, k = 1024, 2048
+    wq, ws = K().quantize_weight_blocks(rand(g, n, k, scale=k ** -0.5))
+    sets = [operands(g, m, 16, k)[:2] for m in (5, 30, 60, 300, 3000)]
+    x = acts(g, 700, k)
+    nw = torch.ones(k, device=DEV)
+
+    def work():
+        outs = [K().gemm_fp8(a, s, wq, ws) for a, s in sets]
+        return outs + [*K().rmsnorm(x, nw, 1e-5, out_dtype=F8), *K().quantize_weight_blocks(x)]
+
+    want = work()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s, kept in zip(streams, got):
+            with torch.cuda.stream(s):
+                kept.append(work())
+    torch.cuda.synchronize()
+    for outs in got[0] + got[1]:
+        for a, b in zip(outs, want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+FIRST_CAPTURED = """
+import torch
+import tjkernels.kernels as K
+torch.manual_seed(0)
+x = torch.randn({rows}, 512, device="cuda")
+w = torch.randn(256, 512, device="cuda")
+nw = torch.ones(512, device="cuda")
+graph = torch.cuda.CUDAGraph()
+
+def work():
+    wq, ws = K.quantize_weight_blocks(w)
+    h, hs = K.rmsnorm(x, nw, 1e-5, out_dtype=torch.float8_e4m3fn)
+    return K.gemm_fp8(h, hs, wq, ws), K.gemm_fp8(*K.quantize_blocks(x), wq, ws)
+
+with torch.cuda.graph(graph):
+    got = work()
+graph.replay()
+for a, b in zip(got, work()):
+    assert a.isfinite().all() and torch.equal(a, b)
+"""
+
+
+@pytest.mark.parametrize("rows", [3, 2000])
+def test_first_calls_of_a_process_captured(rows):
+    """Nothing has to be called once before it can be captured."""
+    import tjkernels
+    path = os.path.dirname(os.path.dirname(tjkernels.__file__))
+    subprocess.run([sys.executable, "-c", FIRST_CAPTURED.format(rows=rows)], check=True,
+                   timeout=120, env={**os.environ, "PYTHONPATH": path})
 
 
 # ------------------------------------------------------------------ refusals

@@ -18,6 +18,8 @@ namespace tjb {
 
 constexpr int kQBlock = 128;      // columns (and weight rows) per scale
 constexpr int kLiveTileRows = 128;  // rows per entry of a live-tile list
+// Longest row: counts of its pieces, rounded up, stay below 2^31.
+constexpr int kMaxColumns = 2147483647 - 1024;
 
 // |v| as an integer: ordered like the magnitude, with NaN above infinity, so
 // an integer maximum propagates both.

@@ -8,9 +8,12 @@
 // read back, scale and add to fp32 sums in registers while the tensor core
 // works on the next block.
 //
-// Up to 64 tokens, in tiles of BT = 16, 32 or 64: the weights are the MMA's 128-row operand
-// (TMEM lane = output column n) and the tokens its N operand, so a few tokens
-// cost a narrow MMA and not a padded one.  The k-blocks of a tile are divided
+// Few tokens, in tiles of BT = 16, 32 or 64: the weights are the MMA's 128-row
+// operand (TMEM lane = output column n) and the tokens its N operand, so a few
+// tokens cost a narrow MMA and not a padded one.  A call of this size is bound
+// by its chain launch -> first loads -> MMA -> meeting, then by reading the
+// weights (M16 N4096 K4096: 7.2 us, floor 2.6; M48 N16384 K4096 with GELU and
+// an 8-bit output: 18 us, floor 10.4).  The k-blocks of a tile are divided
 // over the CTAs of a cluster (so that enough SMs stream the weights), whose
 // fp32 sums meet in distributed shared memory: CTA r finishes the tokens
 // t = r mod c, adding the CTAs' parts in a fixed order.
@@ -1016,8 +1019,8 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
   const bool q = out_dtype == TJB_E4M3;
   if (q && !c_scales) return TJB_ERR_INVALID_ARGUMENT;
   const int unit = q ? 16 : 8;  // output columns: whole 16-byte pieces
-  if (K % 16 != 0 || N % unit != 0 || lda < K || ldw < K || ldc < N ||
-      M > 2147483647 - kLiveTileRows)
+  if (K % 16 != 0 || N % unit != 0 || K > kMaxColumns || N > kMaxColumns || lda < K || ldw < K ||
+      ldc < N || M > 2147483647 - kLiveTileRows)
     return TJB_ERR_BAD_SHAPE;
   auto misaligned4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; };
   if (lda % 16 != 0 || ldw % 16 != 0 || ldc % unit != 0 || !aligned16(A) || !aligned16(W) ||

@@ -190,7 +190,8 @@ int check_quantize(const void* x, int64_t ldx, int in_dtype, const void* q, cons
                    int64_t rows, int K) {
   if (!x || !q || !scales || rows < 0 || K <= 0) return TJB_ERR_INVALID_ARGUMENT;
   if (in_dtype < TJB_F32 || in_dtype > TJB_BF16) return TJB_ERR_UNSUPPORTED_DTYPE;
-  if (K % 16 != 0 || ldx < K || rows > 2147483647 - kLiveTileRows) return TJB_ERR_BAD_SHAPE;
+  if (K % 16 != 0 || K > kMaxColumns || ldx < K || rows > 2147483647 - kLiveTileRows)
+    return TJB_ERR_BAD_SHAPE;
   // Rows start on 16-byte boundaries.
   if (!aligned16(x) || ldx % (in_dtype == TJB_F32 ? 4 : 8) != 0 || !aligned16(q) ||
       (reinterpret_cast<uintptr_t>(scales) & 3u) != 0)

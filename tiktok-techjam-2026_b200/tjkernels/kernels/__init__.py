@@ -446,6 +446,7 @@ def forward_small(model: SmallModel, x: torch.Tensor, valid: Optional[torch.Tens
 
 SCALE_BLOCK = 128
 _E4M3 = torch.float8_e4m3fn
+_INT_MAX = 2 ** 31 - 1  # sizes and pitches pass the C entry points as int
 
 
 def _same_device(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
@@ -482,7 +483,8 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     if t.is_contiguous() and c % unit == 0 and t.data_ptr() % 16 == 0:
         return t, c
     pitch = t.stride(0) if r > 1 else -(-c // unit) * unit
-    if t.stride(1) != 1 or pitch < c or pitch % unit != 0 or t.data_ptr() % 16 != 0:
+    if t.stride(1) != 1 or pitch < c or pitch % unit != 0 or pitch > _INT_MAX \
+            or t.data_ptr() % 16 != 0:
         t = t.clone(memory_format=torch.contiguous_format)
         pitch = c
     return t, pitch
@@ -511,6 +513,8 @@ def quantize_blocks(x: torch.Tensor, m_tiles: Optional[torch.Tensor] = None
         raise ValueError("x must be [R, K]")
     code = _code(x.dtype)
     r, k = x.shape
+    if k > _INT_MAX:
+        raise ValueError("rows of at most 2**31 - 1025 columns")
     tiles = None if m_tiles is None else _check_tiles(m_tiles, device, r)
     q = torch.empty(r, k, dtype=_E4M3, device=device)
     scales = torch.empty(r, (k + 127) // 128, dtype=torch.float32, device=device)
@@ -532,6 +536,8 @@ def quantize_weight_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]
         raise ValueError("w must be [N, K]")
     code = _code(w.dtype)
     n, k = w.shape
+    if k > _INT_MAX:
+        raise ValueError("rows of at most 2**31 - 1025 columns")
     q = torch.empty(n, k, dtype=_E4M3, device=device)
     scales = torch.empty((n + 127) // 128, (k + 127) // 128, dtype=torch.float32, device=device)
     if n:
@@ -568,6 +574,8 @@ def fused_add_rmsnorm(
         raise ValueError("residual must be a contiguous [rows, d] tensor")
     shape = residual.shape
     rows, d = shape
+    if d > _INT_MAX:
+        raise ValueError("rows of at most 16384 columns")
     dtype = residual.dtype
     if weight.dtype != torch.float32 or weight.shape != (d,) or not weight.is_contiguous():
         raise ValueError("weight must be a contiguous fp32 [d] tensor")
@@ -644,6 +652,8 @@ def gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales:
     n, k2 = w.shape
     if k != k2:
         raise ValueError(f"inner dims differ: {k} vs {k2}")
+    if m > _INT_MAX or n > _INT_MAX or k > _INT_MAX:
+        raise ValueError("sizes below 2**31 only")
     if a.dtype != _E4M3 or w.dtype != _E4M3:
         raise TypeError("a and w must be float8_e4m3fn")
     if a_scales.dtype != torch.float32 or w_scales.dtype != torch.float32:
@@ -674,6 +684,8 @@ def gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales:
             raise ValueError("out must be an [M, N] tensor of out_dtype with consecutive columns")
         if m > 1:
             ldc = out.stride(0)
+            if ldc > _INT_MAX:
+                raise ValueError("rows of out less than 2**31 elements apart only")
     if m:
         a, lda = _rows(a)
         w, ldw = _rows(w)
