@@ -303,7 +303,12 @@ GEMM_SHAPES = [(1, 64, 16), (1, 4096, 4096), (2, 136, 128), (15, 384, 1040), (16
                # of two, four and eight; rounds of wide tiles with the rows left
                # over in 64-token tiles, and with the tiles left over split.
                (1900, 1024, 4096), (1000, 1016, 8192), (500, 1024, 16384), (5000, 1024, 4096),
-               (640, 8192, 8192)]
+               (640, 8192, 8192),
+               # Pairs: even and odd counts of 128-row tiles, one and several
+               # chunks of scales, a last tile of 8 columns.
+               (9400, 1032, 656), (9500, 2048, 1168), (4700, 4096, 2064), (11000, 528, 128),
+               # Many columns and one tile of rows: single CTAs.
+               (128, 40000, 256)]
 
 
 @pytest.mark.parametrize("m,n,k", GEMM_SHAPES)

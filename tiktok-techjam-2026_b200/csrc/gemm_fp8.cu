@@ -335,8 +335,9 @@ __global__ void __launch_bounds__(SkinnyCfg<BT>::kThreads)
     }
     // Token t goes to CTA t mod splits, slot t / splits of this CTA's part.
     const int shift = 31 - __clz(splits);
-    const uint32_t mine = smem_u32(sEx) +
-                          static_cast<uint32_t>((rank * (BT >> shift)) * kF8Lanes + quad * 32 + lane) * 4u;
+    const uint32_t mine =
+        smem_u32(sEx) +
+        static_cast<uint32_t>((rank * (BT >> shift)) * kF8Lanes + quad * 32 + lane) * 4u;
 #pragma unroll
     for (int j = 0; j < kCols; ++j) {
       const int t = group * kCols + j;
@@ -427,43 +428,56 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
 }
 
 // ------------------------------------------------------------------------
-// More tokens: 128 x 256 tiles of C.  Here the tokens are the MMA's rows: a
+// More tokens: tiles of 256 columns.  Here the tokens are the MMA's rows: a
 // thread owns one token and 128 consecutive output columns, which is one weight
 // block (one scale product per k-block) and one output block (its 8-bit scale
-// needs no exchange).  Persistent, 384 threads:
+// needs no exchange).  384 threads:
 //   warp 0        TMA producer
-//   warp 1        MMA issuer: per k-block four K = 32 MMAs into
-//                 one of two 256-column TMEM accumulators
-//   warps 2, 3    products sa[m, kb] sw[n / 128, kb] of the tile's rows, four
+//   warp 1        MMA issuer: per k-block four K = 32 MMAs into one of two
+//                 256-column TMEM accumulators
+//   warps 2, 3    products sa[m, kb] sw[n / 128, kb] of the tile's rows, kChunk
 //                 k-blocks at a time, a ring slot ahead of their use, and its
 //                 bias
 //   warps 4..11   two warp groups, 128 columns each: read P_kb from TMEM in
 //                 16-column pieces, the next in flight while one is added to
 //                 128 fp32 sums in registers; then GELU, rounding, and TMA
 //                 stores from a staging buffer of their own
-// Per k-block and SM the tensor core takes 512 clocks (128 x 256 x 128 at
-// 8192 products a clock), the multiply-adds 280 (packed pairs, two clocks a
-// warp).  What bounds it is the chain MMA -> barrier -> scaling -> barrier ->
-// MMA over the two accumulators: every barrier operation, load and spilled
-// register in the k-loop adds to it.  The scaling threads need the registers
-// that warps 0-3 give up (128 x 72 + 256 x 216 = 384 x 168 at launch).  Loads,
-// MMAs and sums together also draw the board's power limit (clocks near 1.45
-// GHz at M16384 N4096 K16384).  A CTA-pair form (two SMs on one 256 x 256
-// tile, a third less L2 traffic) ran the long products as fast and those with
-// K = 1024 a tenth slower: its hand-backs cross SMs.
-//
-// kSplit: the tile's k-blocks are divided over the CTAs of a cluster, for
-// products with too few tiles to fill the SMs.  Each CTA ends with fp32 sums of
-// the whole tile; CTA k finishes rows k * 128 / c ... of it, reading the other
-// CTAs' sums through distributed shared memory and adding them in a fixed
-// order.
+// Three forms:
+//   kPaired  Persistent pairs of SMs (cta_group::2) on tiles of 256 rows, each
+//            SM with 128 rows of A and half of the weights: 32 KB of loads a
+//            k-block and SM where a single one loads 48 KB.
+//   kWhole   Persistent single CTAs on tiles of 128 rows, where the count of
+//            tiles divides better by SMs than by pairs.
+//   kSplitK  128-row tiles whose k-blocks are divided over the CTAs of a
+//            cluster, for too few tiles to fill the SMs.  Each CTA ends with
+//            fp32 sums of the whole tile; CTA k finishes rows k * 128 / c ... of
+//            it, reading the other CTAs' sums through distributed shared
+//            memory and adding them in a fixed order.
+// Per k-block and SM the tensor core takes 512 clocks, the multiply-adds 256
+// (packed pairs, two clocks a warp).  Measured, a k-block of a pair takes 575
+// with MMAs and loads alone, 590 with the reads of tensor memory, 690 with the
+// multiply-adds and 740 with scales from the ring; a single CTA 640 and 850.
+// The chain MMA -> barrier -> scaling -> barrier -> MMA over two accumulators
+// bounds it: every barrier operation and spilled register in the k-loop adds
+// to it.  So the k-loop of the scaling warps is unrolled twice, a pair's scales
+// are handed over eight k-blocks at a time, and one elected thread issues a
+// k-block's MMAs and commits (M8192 N8192 K8192 458 us; four k-blocks a
+// hand-over 470, single CTAs 501, those with a loop that is not unrolled 515;
+// accumulators of 128 columns, for more slack, 487: their MMAs are bound by
+// shared memory).  The scaling threads need the registers that warps 0-3 give
+// up (128 x 72 + 256 x 216 = 384 x 168 at launch).  Under a load that lasts,
+// the board's power limit holds the clock near 1.4 GHz.
+enum WideForm { kWhole, kSplitK, kPaired };
+
+template <int kForm>
 struct WideCfg {
-  static constexpr int kStages = 3;
+  static constexpr int kStages = kForm == kPaired ? 4 : 3;
   static constexpr int kThreads = 384;
   static constexpr uint32_t kABytes = 128 * kF8BK;
-  static constexpr uint32_t kBBytes = 256 * kF8BK;
+  static constexpr uint32_t kBBytes = (kForm == kPaired ? 128 : 256) * kF8BK;
   static constexpr uint32_t kTmemCols = 512;      // two 256-column accumulators
-  static constexpr int kChunk = 4;                // k-blocks of scale products per ring slot
+  // k-blocks of scale products per ring slot
+  static constexpr int kChunk = kForm == kPaired ? 8 : 4;
   // Two ring slots of kChunk x 256 scale products, and two tiles' bias.
   static constexpr uint32_t kScaleBytes = 2 * kChunk * 256 * 4 + 2 * 256 * 4;
   static constexpr uint32_t kOutTile = 32 * 128;  // 32 rows x 128 bytes, 128-byte swizzle
@@ -471,6 +485,60 @@ struct WideCfg {
   static constexpr uint32_t kSmemBytes =
       1024 + kStages * (kABytes + kBBytes) + kOutBytes + kScaleBytes + 256;
 };
+
+// The four K = 32 MMAs of one 128-byte k-block and two commits, all by one
+// elected thread.  The pair's form runs on both CTAs' operands and tensor
+// memory and signals the barriers of both.
+__device__ __forceinline__ void umma_e4m3_block_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                                  uint32_t idesc, uint64_t* bar0, uint64_t* bar1) {
+  asm volatile(
+      "{\n\t.reg .pred e, z;\n\t.reg .b64 a, b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 z, 0, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, z;\n\t"
+      "setp.eq.b32 z, 0, 0;\n\t"
+      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64"
+      " [%4];\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64"
+      " [%5];\n\t}" ::"r"(d_tmem), "l"(adesc),
+      "l"(bdesc), "r"(idesc), "r"(smem_u32(bar0)), "r"(smem_u32(bar1))
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_e4m3_block_pair_w(uint32_t d_tmem, uint64_t adesc,
+                                                       uint64_t bdesc, uint32_t idesc,
+                                                       uint64_t* bar0, uint64_t* bar1) {
+  asm volatile(
+      "{\n\t.reg .pred e, z;\n\t.reg .b64 a, b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 z, 0, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, z;\n\t"
+      "setp.eq.b32 z, 0, 0;\n\t"
+      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%4], %6;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%5], %6;\n\t}" ::"r"(d_tmem), "l"(adesc),
+      "l"(bdesc), "r"(idesc), "r"(smem_u32(bar0)), "r"(smem_u32(bar1)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+// Arrive on the mbarrier at `bar` (shared::cluster address).
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 
 template <int kRegs>
 __device__ __forceinline__ void regs_dec() {
@@ -529,12 +597,13 @@ __device__ __forceinline__ void pull_rows(const GemmF8Args& args, uint32_t half_
   }
 }
 
-template <bool kSplit>
-__global__ void __launch_bounds__(WideCfg::kThreads, 1)
+template <int kForm>
+__global__ void __launch_bounds__(WideCfg<kForm>::kThreads, 1)
     gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmA,
                          const __grid_constant__ CUtensorMap tmB,
                          const __grid_constant__ CUtensorMap tmC, const GemmF8Args args) {
-  using Cfg = WideCfg;
+  using Cfg = WideCfg<kForm>;
+  constexpr bool kSplit = kForm == kSplitK, kPair = kForm == kPaired;
   constexpr int kStages = Cfg::kStages, kChunk = Cfg::kChunk;
   constexpr int BN = 256;
   extern __shared__ uint8_t smem_raw[];
@@ -557,7 +626,7 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = kSplit ? args.splits : 1;
-  const int rank = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+  const int rank = kForm != kWhole ? static_cast<int>(cluster_ctarank()) : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -566,7 +635,7 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 8);  // the scaling warps
+      mbar_init(&tempty[b], kPair ? 16 : 8);  // the scaling warps (of both CTAs)
       mbar_init(&sfull[b], 2);   // warps 2 and 3
       mbar_init(&sempty[b], 8);  // the scaling warps
     }
@@ -578,28 +647,48 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
     prefetch_tmap(&tmC);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, Cfg::kTmemCols);
-    tmem_relinquish();
+    if constexpr (kPair) {
+      tmem_alloc_pair(tmem_slot, Cfg::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, Cfg::kTmemCols);
+      tmem_relinquish();
+    }
   }
   __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  // (A pair: both CTAs' barriers and tensor memory, before either signals.)
+  if constexpr (kPair)
+    cluster_sync();
+  else
+    __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();
   griddep_launch_dependents();
-  const int num_m = args.m_tiles != nullptr ? __ldg(args.m_tiles) : (args.M + 127) / 128;
+  const int num_m1 = args.m_tiles != nullptr ? __ldg(args.m_tiles) : (args.M + 127) / 128;
+  const int num_m = kPair ? (num_m1 + 1) / 2 : num_m1;
   const int num_n = (args.N + BN - 1) / BN;
   const int num_k = (args.K + kF8BK - 1) / kF8BK;
   // Tiles first, first + step, ... below end; k-blocks [k0, k1) of each.
   const int end = min(num_m * num_n, args.end_tile);
-  const int first = args.first_tile + static_cast<int>(blockIdx.x) / splits;
-  const int step = kSplit ? end : static_cast<int>(gridDim.x);  // (kSplit: one tile)
+  const int first = args.first_tile + static_cast<int>(blockIdx.x) / (kPair ? 2 : splits);
+  const int step =  // (kSplit: one tile)
+      kSplit ? end : static_cast<int>(gridDim.x) / (kPair ? 2 : 1);
   const int k0 = kSplit ? rank * num_k / splits : 0;
   const int k1 = kSplit ? (rank + 1) * num_k / splits : num_k;
   auto coords = [&](int t, int& m_blk, int& n_blk) {
     tile_coords(t, num_m, num_n, m_blk, n_blk);
+    bool has = true;
+    if constexpr (kPair) {
+      // This CTA's 128 rows of the pair's 256; where the second 128 do not
+      // exist its CTA loads the first's again (the MMA needs both) and stores
+      // nothing.
+      has = 2 * m_blk + rank < num_m1;
+      m_blk = 2 * m_blk + (has ? rank : 0);
+    }
     if (args.m_tiles != nullptr) m_blk = __ldg(args.m_tiles + 1 + m_blk);
+    return has;
   };
 
   if (warp < 4) {
@@ -608,6 +697,7 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
       // ------------------------------------------------------------ producer
       int stage = 0;
       uint32_t phase = 0, issued = 0, last_parity = 0;
+      const uint32_t full_at = kPair ? map_to_rank(smem_u32(full), 0) : 0u;  // (the leader's)
       bool ok = true;
       for (int t = first; ok && t < end; t += step) {
         int m_blk, n_blk;
@@ -617,9 +707,17 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[stage], Cfg::kABytes + Cfg::kBBytes);
-          tma_load_2d(sA + stage * Cfg::kABytes, &tmA, &full[stage], kb * kF8BK, m_blk * 128);
-          tma_load_2d(sB + stage * Cfg::kBBytes, &tmB, &full[stage], kb * kF8BK, n_blk * BN);
+          if constexpr (kPair) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (Cfg::kABytes + Cfg::kBBytes));
+            const uint32_t bar = full_at + static_cast<uint32_t>(stage) * 8u;
+            tma_load_2d_pair(sA + stage * Cfg::kABytes, &tmA, bar, kb * kF8BK, m_blk * 128);
+            tma_load_2d_pair(sB + stage * Cfg::kBBytes, &tmB, bar, kb * kF8BK,
+                             n_blk * BN + rank * 128);
+          } else {
+            mbar_arrive_expect_tx(&full[stage], Cfg::kABytes + Cfg::kBBytes);
+            tma_load_2d(sA + stage * Cfg::kABytes, &tmA, &full[stage], kb * kF8BK, m_blk * 128);
+            tma_load_2d(sB + stage * Cfg::kBBytes, &tmB, &full[stage], kb * kF8BK, n_blk * BN);
+          }
           issued |= 1u << stage;
           last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
           if (++stage == kStages) {
@@ -628,41 +726,43 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
           }
         }
       }
-      // Every load has landed before the CTA may release its memory.
+      // Every load has landed before the CTA may release its memory (a pair's
+      // loads count on the leader's barrier: their stage has been read).
       for (int s = 0; s < kStages; ++s)
-        if ((issued >> s) & 1u) mbar_wait_drain(&full[s], (last_parity >> s) & 1u);
-    } else if (warp == 1) {
+        if ((issued >> s) & 1u)
+          mbar_wait_drain(kPair ? &empty[s] : &full[s], (last_parity >> s) & 1u);
+    } else if (warp == 1 && (!kPair || rank == 0)) {
       // ---------------------------------------------------------- MMA issuer
-      constexpr uint32_t idesc = idesc_e4m3(128, BN);
+      constexpr uint32_t idesc = idesc_e4m3(kPair ? 256 : 128, BN);
       int stage = 0;
       uint32_t phase = 0, it = 0;
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
-      };
-      for (int t = first; ok && t < end; t += step) {
+      for (int t = first; t < end; t += step) {
         for (int kb = k0; kb < k1; ++kb, ++it) {
           const uint32_t acc = it & 1;
-          if (!wait(&full[stage], phase) || !wait(&tempty[acc], ((it >> 1) & 1) ^ 1)) {
-            ok = false;
-            break;
-          }
+          // (A wait that ran out has recorded its status and raised the abort
+          // flag, which ends all later ones: the loop runs on to its end.)
+          mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1, abort_flag);
+          mbar_wait(&full[stage], phase, abort_flag);
+          __syncwarp();
           tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + stage * Cfg::kABytes);
-          const uint32_t b0 = smem_u32(sB + stage * Cfg::kBBytes);
-#pragma unroll
-          for (int k = 0; k < kF8BK / 32; ++k)
-            umma_e4m3_w(tmem_base + acc * BN, sdesc_sw128(a0 + k * 32, 16, 1024),
-                        sdesc_sw128(b0 + k * 32, 16, 1024), idesc, k > 0 ? 1u : 0u);
-          umma_commit_w(&tfull[acc]);
-          umma_commit_w(&empty[stage]);
+          const uint64_t a_desc = sdesc_sw128(smem_u32(sA + stage * Cfg::kABytes), 16, 1024);
+          const uint64_t b_desc = sdesc_sw128(smem_u32(sB + stage * Cfg::kBBytes), 16, 1024);
+          if constexpr (kPair)
+            umma_e4m3_block_pair_w(tmem_base + acc * BN, a_desc, b_desc, idesc, &tfull[acc],
+                                   &empty[stage]);
+          else
+            umma_e4m3_block_w(tmem_base + acc * BN, a_desc, b_desc, idesc, &tfull[acc],
+                              &empty[stage]);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      umma_commit_w(drain);
+      if constexpr (kPair)
+        umma_commit_pair_w(drain, 0x1);
+      else
+        umma_commit_w(drain);
       mbar_wait_drain(drain, 0);
     } else if (warp >= 2) {
       // ------------------------------------------------------- scales and bias
@@ -696,38 +796,37 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
           bias = b;
         }
         for (int kb0 = k0; ok && kb0 < k1; kb0 += kChunk, ++c) {
-          float va[kChunk], vb[kChunk];
-          if (vec && kb0 % 4 == 0 && kb0 + kChunk <= k1) {
-#pragma unroll
-            for (int u = 0; u < kChunk; u += 4) {
-              *reinterpret_cast<float4*>(va + u) =
-                  __ldg(reinterpret_cast<const float4*>(a0 + kb0 + u));
-              *reinterpret_cast<float4*>(vb + u) =
-                  __ldg(reinterpret_cast<const float4*>(a1 + kb0 + u));
-            }
-          } else {
-#pragma unroll
-            for (int u = 0; u < kChunk; ++u) {
-              const int kb = min(kb0 + u, k1 - 1);
-              va[u] = __ldg(a0 + kb * args.as_blk);
-              vb[u] = __ldg(a1 + kb * args.as_blk);
-            }
-          }
-          float s0[kChunk], s1[kChunk];
-#pragma unroll
-          for (int u = 0; u < kChunk; ++u) {
-            s0[u] = __ldg(w0 + min(kb0 + u, k1 - 1));
-            s1[u] = __ldg(w1 + min(kb0 + u, k1 - 1));
-          }
           ok = __all_sync(0xffffffffu,
                           mbar_wait(&sempty[c & 1], ((c >> 1) & 1) ^ 1, abort_flag));
-          float* dst = sScale + (c & 1) * kChunk * 256 + r;
+#pragma unroll 1
+          for (int v = 0; v < kChunk && kb0 + v < k1; v += 4) {
+            const int kv = kb0 + v;
+            float va[4], vb[4];
+            if (vec && kv % 4 == 0 && kv + 4 <= k1) {
+              *reinterpret_cast<float4*>(va) = __ldg(reinterpret_cast<const float4*>(a0 + kv));
+              *reinterpret_cast<float4*>(vb) = __ldg(reinterpret_cast<const float4*>(a1 + kv));
+            } else {
 #pragma unroll
-          for (int u = 0; u < kChunk; ++u) {
-            dst[u * 256] = va[u] * s0[u];
-            dst[u * 256 + 32] = vb[u] * s0[u];
-            dst[u * 256 + 128] = va[u] * s1[u];
-            dst[u * 256 + 160] = vb[u] * s1[u];
+              for (int u = 0; u < 4; ++u) {
+                const int kb = min(kv + u, k1 - 1);
+                va[u] = __ldg(a0 + kb * args.as_blk);
+                vb[u] = __ldg(a1 + kb * args.as_blk);
+              }
+            }
+            float s0[4], s1[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              s0[u] = __ldg(w0 + min(kv + u, k1 - 1));
+              s1[u] = __ldg(w1 + min(kv + u, k1 - 1));
+            }
+            float* dst = sScale + ((c & 1) * kChunk + v) * 256 + r;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              dst[u * 256] = va[u] * s0[u];
+              dst[u * 256 + 32] = vb[u] * s0[u];
+              dst[u * 256 + 128] = va[u] * s1[u];
+              dst[u * 256 + 160] = vb[u] * s1[u];
+            }
           }
           if (!kSplit && kb0 == k0) {
             reinterpret_cast<float4*>(sBias + odd * 256)[(warp - 2) * 32 + lane] = bias;
@@ -752,18 +851,19 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
     uint8_t* buf = sOut + (warp - 4) * 2 * Cfg::kOutTile;
     const uint32_t taddr0 =
         tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 128);
+    const uint32_t tempty_at = kPair ? map_to_rank(smem_u32(tempty), 0) : 0u;  // (the leader's)
     uint32_t it = 0, chunk = 0;  // k-blocks and scale chunks done, over all tiles
     uint32_t odd = 0;            // tiles done, parity
     bool ok = true;
     bool met = !kSplit;  // this warp has been at the cluster's two meetings
     for (int t = first; ok && t < end; t += step) {
       int m_blk, n_blk;
-      coords(t, m_blk, n_blk);
+      const bool has = coords(t, m_blk, n_blk);
       const int n0 = n_blk * BN + half * 128;
       // The sums start from the bias, which comes with the first scales;
       // columns past N stay exactly zero (their weight rows load as zeros), as
       // a ragged 8-bit block's scale needs.
-      ok = mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag) && ok;
+      mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag);
       float sum[128];
 #pragma unroll
       for (int j = 0; j < 128; j += 4) {
@@ -775,14 +875,14 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
         sum[j + 3] = b.w;
       }
       odd ^= 1;
-#pragma unroll 1
+#pragma unroll 2
       for (int kb = k0; kb < k1; ++kb, ++it) {
         const int u = (kb - k0) & (kChunk - 1);
         if (u == 0 && kb > k0)
-          ok = mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag) && ok;
+          mbar_wait(&sfull[chunk & 1], (chunk >> 1) & 1, abort_flag);
         const float s = sScale[((chunk & 1) * kChunk + u) * 256 + half * 128 + r];
         const uint32_t acc = it & 1;
-        ok = mbar_wait(&tfull[acc], (it >> 1) & 1, abort_flag) && ok;
+        mbar_wait(&tfull[acc], (it >> 1) & 1, abort_flag);
         __syncwarp();
         tc_fence_after();
         const uint32_t taddr = taddr0 + acc * BN;
@@ -798,13 +898,16 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&tempty[acc]);
+          if constexpr (kPair)
+            mbar_arrive_at(tempty_at + acc * 8u);
+          else
+            mbar_arrive(&tempty[acc]);
           if (u == kChunk - 1 || kb == k1 - 1) mbar_arrive(&sempty[chunk & 1]);
         }
         if (u == kChunk - 1 || kb == k1 - 1) ++chunk;
         add_scaledN(sum + 128 - 16, p[1], s);
       }
-      ok = __all_sync(0xffffffffu, ok);
+      ok = __all_sync(0xffffffffu, *abort_flag == 0);
       if constexpr (kSplit) {
         // The sums go to this CTA's shared memory as [half][row][32 chunks of
         // 16 bytes, chunk j at j ^ (row & 31)] (the stage ring: this thread
@@ -837,7 +940,7 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
         break;
       }
       if (!ok) break;
-      if (n0 >= args.N) continue;  // warp-uniform
+      if (n0 >= args.N || !has) continue;  // warp-uniform
       if (args.act == 1) {
 #pragma unroll
         for (int j = 0; j < 128; j += 2) gelu_pair(sum[j], sum[j + 1]);
@@ -915,17 +1018,26 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
 
   __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  // (A pair: neither CTA leaves while the other or the MMAs may still touch
+  // its barriers, operands or tensor memory.)
+  if constexpr (kPair)
+    cluster_sync();
+  else
+    __syncthreads();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    if constexpr (kPair)
+      tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    else
+      tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
 }
 
 // Clusters of 1, 2, 4 and 8 CTAs that run at once, per device.
 struct WideLimits {
   int clusters[4];
+  int pairs;
   bool known;
 };
 WideLimits g_f8_wide[64];
@@ -937,66 +1049,82 @@ int wide_limits(WideLimits& lim) {
   std::lock_guard<std::mutex> lock(g_f8_mu);
   WideLimits& l = g_f8_wide[dev];
   if (!l.known) {
-    for (auto kern : {gemm_fp8_wide_kernel<false>, gemm_fp8_wide_kernel<true>})
+    const uint32_t bytes[3] = {WideCfg<kWhole>::kSmemBytes, WideCfg<kSplitK>::kSmemBytes,
+                               WideCfg<kPaired>::kSmemBytes};
+    const decltype(&gemm_fp8_wide_kernel<kWhole>) kernels[3] = {gemm_fp8_wide_kernel<kWhole>,
+                                                       gemm_fp8_wide_kernel<kSplitK>,
+                                                       gemm_fp8_wide_kernel<kPaired>};
+    for (int i = 0; i < 3; ++i)
       if (const int fs = cuda_status(cudaFuncSetAttribute(
-              kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-              static_cast<int>(WideCfg::kSmemBytes))))
+              kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes[i]))))
         return fs;
     l.clusters[0] = num_sms();
-    for (int i = 1; i < 4; ++i) {
+    auto resident = [&](WideForm form, int log2, int* clusters) {
       cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(static_cast<unsigned>(num_sms() >> i << i));
-      cfg.blockDim = dim3(WideCfg::kThreads);
-      cfg.dynamicSmemBytes = WideCfg::kSmemBytes;
+      cfg.gridDim = dim3(static_cast<unsigned>(num_sms() >> log2 << log2));
+      cfg.blockDim = dim3(WideCfg<kWhole>::kThreads);
+      cfg.dynamicSmemBytes = bytes[form];
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 1u << i;
+      attr[0].val.clusterDim.x = 1u << log2;
       attr[0].val.clusterDim.y = 1;
       attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      if (const int qs = cuda_status(cudaOccupancyMaxActiveClusters(
-              &l.clusters[i], gemm_fp8_wide_kernel<true>, &cfg)))
-        return qs;
-    }
+      return cuda_status(cudaOccupancyMaxActiveClusters(clusters, kernels[form], &cfg));
+    };
+    for (int i = 1; i < 4; ++i)
+      if (const int qs = resident(kSplitK, i, &l.clusters[i])) return qs;
+    if (const int qs = resident(kPaired, 1, &l.pairs)) return qs;
     l.known = true;
   }
   lim = l;
   return TJB_OK;
 }
 
-// The first `whole` tiles in rounds of one per SM; the others, if any, with
-// their k-blocks split over clusters of 1 << log2 CTAs.
-int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw, int whole,
-                int log2, cudaStream_t stream) {
-  using Cfg = WideCfg;
+// All tiles in pairs (pairs > 0: that many at once); or the first `whole` tiles
+// in rounds of one per SM and the others, if any, with their k-blocks split over
+// clusters of 1 << log2 CTAs.
+int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw, int pairs,
+                int whole, int log2, cudaStream_t stream) {
+  constexpr int kThreads = WideCfg<kWhole>::kThreads;
   CUtensorMap tmA, tmB, tmC;
   int st = make_tmap_2d(&tmA, TJB_E4M3, A, args.K, args.M, lda, kF8BK, 128);
   if (st != TJB_OK) return st;
-  st = make_tmap_2d(&tmB, TJB_E4M3, W, args.K, args.N, ldw, kF8BK, 256);
+  st = make_tmap_2d(&tmB, TJB_E4M3, W, args.K, args.N, ldw, kF8BK,
+                    pairs > 0 ? 128 : 256);
   if (st != TJB_OK) return st;
   const int esz = args.out_dtype == TJB_F32 ? 4 : args.out_dtype == TJB_E4M3 ? 1 : 2;
   st = make_tmap_2d(&tmC, args.out_dtype, args.C, args.N, args.M,
                     static_cast<uint64_t>(args.ldc) * esz, 128 / esz, 32);
   if (st != TJB_OK) return st;
-  const int tiles = (args.M + 127) / 128 * ((args.N + 255) / 256);
+  const int wide_n = (args.N + 255) / 256;
+  args.splits = 1;
+  if (pairs > 0) {
+    const int tiles = (args.M + 255) / 256 * wide_n;
+    args.first_tile = 0;
+    args.end_tile = tiles;
+    return launch_kernel_cluster(gemm_fp8_wide_kernel<kPaired>,
+                                 dim3(2u * static_cast<unsigned>(tiles < pairs ? tiles : pairs)),
+                                 dim3(kThreads), WideCfg<kPaired>::kSmemBytes, stream, 2u, tmA, tmB,
+                                 tmC, args);
+  }
+  const int tiles = (args.M + 127) / 128 * wide_n;
   const int sms = num_sms();
   if (whole > 0) {
     args.first_tile = 0;
     args.end_tile = whole;
-    args.splits = 1;
-    const int grid = whole < sms ? whole : sms;
-    st = launch_kernel(gemm_fp8_wide_kernel<false>, dim3(grid), dim3(Cfg::kThreads),
-                       Cfg::kSmemBytes, stream, tmA, tmB, tmC, args);
+    st = launch_kernel(gemm_fp8_wide_kernel<kWhole>, dim3(whole < sms ? whole : sms),
+                       dim3(kThreads), WideCfg<kWhole>::kSmemBytes, stream, tmA, tmB, tmC, args);
     if (st != TJB_OK) return st;
   }
   if (whole < tiles) {
     args.first_tile = whole;
     args.end_tile = tiles;
     args.splits = 1 << log2;
-    st = launch_kernel_cluster(gemm_fp8_wide_kernel<true>,
-                               dim3(static_cast<unsigned>(tiles - whole) << log2),
-                               dim3(Cfg::kThreads), Cfg::kSmemBytes, stream,
+    st = launch_kernel_cluster(gemm_fp8_wide_kernel<kSplitK>,
+                               dim3(static_cast<unsigned>(tiles - whole) << log2), dim3(kThreads),
+                               WideCfg<kSplitK>::kSmemBytes, stream,
                                static_cast<unsigned>(args.splits), tmA, tmB, tmC, args);
   }
   return st;
@@ -1050,10 +1178,10 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
   if (M <= 32) return launch_skinny<32>(A, W, args, lda, ldw, s);
   if (M <= 64) return launch_skinny<64>(A, W, args, lda, ldw, s);
   // More: 64-token tiles (quick to start, their parts quick to meet, but the
-  // tensor core a third as busy) or wide ones (in rounds of one per SM, or
-  // split over clusters, or both), by the time that each is expected to take.
-  // The constants, in us, were fitted to 60 shapes of M 65-8000, N 128-8192, K
-  // 128-8192 on a B200 (mean error 7-9 %); the choice comes within 1 % of the
+  // tensor core a third as busy) or wide ones (pairs, single CTAs, or split over
+  // clusters), or wide ones and the rest, by the time that each is expected to
+  // take.  The constants, in us, were fitted to shapes of M 65-16384, N 128-8192,
+  // K 128-16384 on a B200 (mean error 7-9 %); the choice comes within 1 % of the
   // best of the forms on average, 28 % at worst.
   WideLimits lim;
   if (const int st = wide_limits(lim)) return st;
@@ -1066,35 +1194,55 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
     const double t = static_cast<double>((m + 63) / 64 * num_n);
     return 4.3 + t * (0.0157 + 0.0024 * num_k);
   };
-  auto wide_us = [&](int64_t rounds) { return 2.9 + rounds * (0.53 * num_k + 1.75); };
-  const int64_t rounds = (tiles + sms - 1) / sms;
+  auto whole_us = [&](int64_t rounds) { return 2.9 + rounds * (0.52 * num_k + 1.75); };
+  // m rows in wide tiles without a split, and the pairs for it (0: single CTAs).
+  auto wide_us = [&](int64_t m, int& pairs) {
+    const int64_t m1 = (m + 127) / 128, m2 = (m + 255) / 256;
+    const double single = whole_us((m1 * wide_n + sms - 1) / sms);
+    pairs = 0;
+    if (lim.pairs <= 0) return single;
+    const int64_t rounds = (m2 * wide_n + lim.pairs - 1) / lim.pairs;
+    const double paired = 3.4 + rounds * (0.49 * num_k + 1.7);
+    if (paired >= single) return single;
+    pairs = lim.pairs;
+    return paired;
+  };
   double best = skinny_us(M);
   enum { kSkinny, kWide, kRows } form = kSkinny;
-  int whole = static_cast<int>(tiles), log2 = 0;
-  if (wide_us(rounds) < best) {
-    best = wide_us(rounds);
+  int whole = static_cast<int>(tiles), log2 = 0, pairs = 0;
+  const double wide = wide_us(M, pairs);
+  if (wide < best) {
+    best = wide;
     form = kWide;
   }
   // The last, partial round: split, or its rows in 64-token tiles.
+  const int64_t rounds = (tiles + sms - 1) / sms;
   const int64_t full = (rounds - 1) * sms;
-  const double full_us = rounds > 1 ? wide_us(rounds - 1) : 0.0;
+  const double full_us = rounds > 1 ? whole_us(rounds - 1) : 0.0;
   for (int i = 1; i < 4 && 1 << i <= num_k && tiles - full <= lim.clusters[i]; ++i) {
     const double us = full_us + 8.9 + 0.66 * num_k / (1 << i);
     if (us < best) {
       best = us;
       form = kWide;
+      pairs = 0;
       whole = static_cast<int>(full);
       log2 = i;
     }
   }
   const int64_t rows = full / wide_n * 128;  // (a live-tile list is not cut)
-  if (rows > 0 && m_tiles == nullptr && full_us + 1.5 + skinny_us(M - rows) < best) form = kRows;
+  if (rows > 0 && m_tiles == nullptr) {
+    int rows_pairs = 0;
+    if (wide_us(rows, rows_pairs) + 1.5 + skinny_us(M - rows) < best) {
+      form = kRows;
+      pairs = rows_pairs;
+    }
+  }
   if (form == kSkinny) return launch_skinny<64>(A, W, args, lda, ldw, s);
-  if (form == kWide) return launch_wide(A, W, args, lda, ldw, whole, log2, s);
+  if (form == kWide) return launch_wide(A, W, args, lda, ldw, pairs, whole, log2, s);
   const int esz = out_dtype == TJB_F32 ? 4 : q ? 1 : 2;
   args.M = static_cast<int>(rows);
   whole = static_cast<int>(rows / 128 * wide_n);
-  if (const int st = launch_wide(A, W, args, lda, ldw, whole, 0, s)) return st;
+  if (const int st = launch_wide(A, W, args, lda, ldw, pairs, whole, 0, s)) return st;
   args.M = static_cast<int>(M - rows);
   args.a_scales += rows * a_scales_row;
   args.C = static_cast<uint8_t*>(C) + rows * ldc * esz;
