@@ -677,8 +677,25 @@ __global__ void __launch_bounds__(WideCfg<kForm>::kThreads, 1)
       kSplit ? end : static_cast<int>(gridDim.x) / (kPair ? 2 : 1);
   const int k0 = kSplit ? rank * num_k / splits : 0;
   const int k1 = kSplit ? (rank + 1) * num_k / splits : num_k;
+  // (The order of tile_coords.  Tiles only grow for each role, so the group is
+  // counted up, and in a full group the division is a shift: 400 clocks of each
+  // tile's start otherwise; M8192 N8192 K1024 82 -> 79 us.)
+  int group = kSplit ? first / (kGroupM * num_n) : 0;
+  int group_end = (group + 1) * kGroupM * num_n;
   auto coords = [&](int t, int& m_blk, int& n_blk) {
-    tile_coords(t, num_m, num_n, m_blk, n_blk);
+    while (t >= group_end) {
+      ++group;
+      group_end += kGroupM * num_n;
+    }
+    const int r = t - (group_end - kGroupM * num_n);
+    const int gsize = num_m - group * kGroupM;
+    if (gsize >= kGroupM) {
+      m_blk = group * kGroupM + r % kGroupM;
+      n_blk = r / kGroupM;
+    } else {
+      m_blk = group * kGroupM + r % gsize;
+      n_blk = r / gsize;
+    }
     bool has = true;
     if constexpr (kPair) {
       // This CTA's 128 rows of the pair's 256; where the second 128 do not
