@@ -243,8 +243,9 @@ __device__ __forceinline__ void store8(void* out, int dtype, int64_t idx, const 
   }
   uint4 raw;
   if (dtype == TJB_BF16)
-    raw = make_uint4(Pack2<__nv_bfloat16>::pack(y[0], y[1]), Pack2<__nv_bfloat16>::pack(y[2], y[3]),
-                     Pack2<__nv_bfloat16>::pack(y[4], y[5]), Pack2<__nv_bfloat16>::pack(y[6], y[7]));
+    raw = make_uint4(
+        Pack2<__nv_bfloat16>::pack(y[0], y[1]), Pack2<__nv_bfloat16>::pack(y[2], y[3]),
+        Pack2<__nv_bfloat16>::pack(y[4], y[5]), Pack2<__nv_bfloat16>::pack(y[6], y[7]));
   else
     raw = make_uint4(Pack2<__half>::pack(y[0], y[1]), Pack2<__half>::pack(y[2], y[3]),
                      Pack2<__half>::pack(y[4], y[5]), Pack2<__half>::pack(y[6], y[7]));

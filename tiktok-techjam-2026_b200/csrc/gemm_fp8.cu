@@ -503,11 +503,10 @@ __device__ __forceinline__ void umma_e4m3_block_w(uint32_t d_tmem, uint64_t ades
       "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
       "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64"
-      " [%4];\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64"
-      " [%5];\n\t}" ::"r"(d_tmem), "l"(adesc),
-      "l"(bdesc), "r"(idesc), "r"(smem_u32(bar0)), "r"(smem_u32(bar1))
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}" ::
+          "r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(smem_u32(bar0)), "r"(smem_u32(bar1))
       : "memory");
 }
 
@@ -529,9 +528,8 @@ __device__ __forceinline__ void umma_e4m3_block_pair_w(uint32_t d_tmem, uint64_t
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
       " [%4], %6;\n\t"
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-      " [%5], %6;\n\t}" ::"r"(d_tmem), "l"(adesc),
-      "l"(bdesc), "r"(idesc), "r"(smem_u32(bar0)), "r"(smem_u32(bar1)),
-      "h"(static_cast<uint16_t>(3))
+      " [%5], %6;\n\t}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc),
+      "r"(smem_u32(bar0)), "r"(smem_u32(bar1)), "h"(static_cast<uint16_t>(3))
       : "memory");
 }
 
@@ -754,10 +752,11 @@ __global__ void __launch_bounds__(WideCfg<kForm>::kThreads, 1)
       int stage = 0;
       uint32_t phase = 0, it = 0;
       for (int t = first; t < end; t += step) {
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
         for (int kb = k0; kb < k1; ++kb, ++it) {
           const uint32_t acc = it & 1;
           // (A wait that ran out has recorded its status and raised the abort
-          // flag, which ends all later ones: the loop runs on to its end.)
+          // flag, which ends all later ones: the tile runs on to its end.)
           mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1, abort_flag);
           mbar_wait(&full[stage], phase, abort_flag);
           __syncwarp();
