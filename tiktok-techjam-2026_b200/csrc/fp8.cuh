@@ -1,5 +1,5 @@
 // fp8.cuh -- block-scaled e4m3: the quantisation rule, packing, and the
-// 8-bit form of the tensor-core instruction, shared by rmsnorm.cu,
+// instruction descriptor of the 8-bit MMA, shared by rmsnorm.cu,
 // quantize.cu and gemm_fp8.cu.
 //
 // A block of values y (1 x 128 along a row for activations, 128 x 128 for
@@ -256,19 +256,6 @@ __device__ __forceinline__ void store8(void* out, int dtype, int64_t idx, const 
 // accumulation, both K-major; the fields sit as in idesc_f16.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
   return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
-}
-
-// D[tmem] (+)= A[smem] * B[smem] over K = 32 e4m3 columns; warp-collective
-// like umma_ss_w.
-__device__ __forceinline__ void umma_e4m3_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                            uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
 }
 
 }  // namespace tjb

@@ -96,6 +96,53 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
   return v;
 }
 
+// The four K = 32 MMAs of one 128-byte k-block and two commits, all by one
+// elected thread.  The pair's form runs on both CTAs' operands and tensor
+// memory and signals the barriers of both.
+__device__ __forceinline__ void umma_e4m3_block_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                                  uint32_t idesc, uint64_t* bar0, uint64_t* bar1) {
+  asm volatile(
+      "{\n\t.reg .pred e, z;\n\t.reg .b64 a, b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 z, 0, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, z;\n\t"
+      "setp.eq.b32 z, 0, 0;\n\t"
+      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}" ::
+          "r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(smem_u32(bar0)), "r"(smem_u32(bar1))
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_e4m3_block_pair_w(uint32_t d_tmem, uint64_t adesc,
+                                                       uint64_t bdesc, uint32_t idesc,
+                                                       uint64_t* bar0, uint64_t* bar1) {
+  asm volatile(
+      "{\n\t.reg .pred e, z;\n\t.reg .b64 a, b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 z, 0, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, z;\n\t"
+      "setp.eq.b32 z, 0, 0;\n\t"
+      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%4], %6;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%5], %6;\n\t}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc),
+      "r"(smem_u32(bar0)), "r"(smem_u32(bar1)), "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
 template <int kThreads>
 __device__ __forceinline__ void scaling_warps_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
@@ -242,15 +289,10 @@ __global__ void __launch_bounds__(SkinnyCfg<BT>::kThreads)
       if (!wait(&tempty[acc], acc_phase ^ 1)) break;
       if (!wait(&full[stage], phase)) break;
       tc_fence_after();
-      const uint32_t w0 = smem_u32(sW + stage * Cfg::kWBytes);
-      const uint32_t x0 = smem_u32(sX + stage * Cfg::kXBytes);
-      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BT);
-#pragma unroll
-      for (int k = 0; k < kF8BK / 32; ++k)
-        umma_e4m3_w(d_tmem, sdesc_sw128(w0 + k * 32, 16, 1024), sdesc_sw128(x0 + k * 32, 16, 1024),
-                    idesc, k > 0 ? 1u : 0u);
-      umma_commit_w(&empty[stage]);
-      umma_commit_w(&tfull[acc]);
+      umma_e4m3_block_w(tmem_base + static_cast<uint32_t>(acc * BT),
+                        sdesc_sw128(smem_u32(sW + stage * Cfg::kWBytes), 16, 1024),
+                        sdesc_sw128(smem_u32(sX + stage * Cfg::kXBytes), 16, 1024), idesc,
+                        &tfull[acc], &empty[stage]);
       if (++stage == kStages) {
         stage = 0;
         phase ^= 1;
@@ -485,53 +527,6 @@ struct WideCfg {
   static constexpr uint32_t kSmemBytes =
       1024 + kStages * (kABytes + kBBytes) + kOutBytes + kScaleBytes + 256;
 };
-
-// The four K = 32 MMAs of one 128-byte k-block and two commits, all by one
-// elected thread.  The pair's form runs on both CTAs' operands and tensor
-// memory and signals the barriers of both.
-__device__ __forceinline__ void umma_e4m3_block_w(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                                  uint32_t idesc, uint64_t* bar0, uint64_t* bar1) {
-  asm volatile(
-      "{\n\t.reg .pred e, z;\n\t.reg .b64 a, b;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 z, 0, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, z;\n\t"
-      "setp.eq.b32 z, 0, 0;\n\t"
-      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
-      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
-      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}" ::
-          "r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(smem_u32(bar0)), "r"(smem_u32(bar1))
-      : "memory");
-}
-
-__device__ __forceinline__ void umma_e4m3_block_pair_w(uint32_t d_tmem, uint64_t adesc,
-                                                       uint64_t bdesc, uint32_t idesc,
-                                                       uint64_t* bar0, uint64_t* bar1) {
-  asm volatile(
-      "{\n\t.reg .pred e, z;\n\t.reg .b64 a, b;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 z, 0, 0;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, z;\n\t"
-      "setp.eq.b32 z, 0, 0;\n\t"
-      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
-      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
-      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, z;\n\t"
-      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-      " [%4], %6;\n\t"
-      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-      " [%5], %6;\n\t}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc),
-      "r"(smem_u32(bar0)), "r"(smem_u32(bar1)), "h"(static_cast<uint16_t>(3))
-      : "memory");
-}
 
 // Arrive on the mbarrier at `bar` (shared::cluster address).
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
