@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     if (col - (t & 31) * 8 >= d) break;  // warp-uniform
     float y[8] = {};
     if (col < d) {
-      if (kDelta && res_out != nullptr) store8(res_out, res_dtype, base + col, v[i]);
+      if (res_out != nullptr) store8(res_out, res_dtype, base + col, v[i]);
       if (keep) {
         const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + col));
         const float4 w1 = __ldg(reinterpret_cast<const float4*>(w + col) + 1);
@@ -247,6 +247,7 @@ extern "C" int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out
     return TJB_ERR_BAD_ALIGNMENT;
   if (!device_ok()) return TJB_ERR_NO_DEVICE;
   if (rows == 0) return TJB_OK;
+  if (!delta && res_out == res) res_out = nullptr;  // x is there already
   const int64_t n = m_tiles ? (rows + kLiveTileRows - 1) / kLiveTileRows * kLiveTileRows : rows;
   // 16-byte accesses where the types and the alignment allow them.
   const bool vec8 = res_dtype != TJB_F32 && (!delta || delta_dtype == res_dtype) && d % 8 == 0 &&

@@ -567,7 +567,8 @@ def fused_add_rmsnorm(
     ``(q, scales)`` of :func:`quantize_blocks`, computed from the unrounded
     norm (d a multiple of 16; otherwise of 4; at most 16384).
     ``write_residual``, ``residual_out`` (may be ``residual``), ``row_mask``
-    and ``m_tiles`` as in :func:`fused_add_layernorm`."""
+    and ``m_tiles`` as in :func:`fused_add_layernorm`; a ``residual_out`` that
+    is given without a ``delta`` receives ``residual``."""
     device = residual.device
     _same_device(device, delta, weight)
     if residual.dim() != 2 or not residual.is_contiguous():
@@ -608,15 +609,15 @@ def fused_add_rmsnorm(
         out_code = _code(out_dtype)
     out = torch.empty(rows, d, dtype=out_dtype, device=device)
     new, new_at = residual, None
-    if write_residual and delta is not None:
-        if residual_out is None:
-            new = torch.empty_like(residual)
-        else:
-            _same_device(device, residual_out)
-            if residual_out.shape != shape or residual_out.dtype != dtype \
-                    or not residual_out.is_contiguous():
-                raise ValueError("residual_out must be contiguous, of residual's shape and dtype")
-            new = residual_out
+    if write_residual and residual_out is not None:
+        _same_device(device, residual_out)
+        if residual_out.shape != shape or residual_out.dtype != dtype \
+                or not residual_out.is_contiguous():
+            raise ValueError("residual_out must be contiguous, of residual's shape and dtype")
+        new = residual_out
+        new_at = new.data_ptr()
+    elif write_residual and delta is not None:
+        new = torch.empty_like(residual)
         new_at = new.data_ptr()
     if rows:
         _launch("tjb_add_rmsnorm", device, residual.data_ptr(), delta_at, new_at, out.data_ptr(),
