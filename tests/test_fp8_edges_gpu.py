@@ -2,10 +2,13 @@
 that a call has to write, values at the ends of the number range, sizes at the
 ends of the index range.  Against 64-bit formulas, as in test_fp8_gpu.py."""
 
+import math
+
 import pytest
 import torch
 
-from test_fp8_gpu import DEV, NORM_REL, K, check_out, gen, rand, rms_ref
+from test_fp8_gpu import (DEV, F8, NORM_REL, U32, K, check_out, check_quantised, gen, operands,
+                          per_block, rand, rms_ref)
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +58,127 @@ def test_residual_out_without_a_delta_is_checked():
     for bad in (x.half(), x[:2], torch.zeros(32, 4, device=DEV).t()):
         with pytest.raises(ValueError):
             K().fused_add_rmsnorm(x, None, w, 1e-5, residual_out=bad)
+
+
+# ------------------------------------------------------------------------ GELU
+
+# One size of each form of the product: 16, 32 and 64 tokens, wide tiles whose
+# k-blocks are split, whole, in pairs, and with rows left over.
+GELU_ROWS = [1, 20, 40, 100, 700, 5000, 11000]
+
+
+def gelu_of(x, m, dtype):
+    """The product's GELU of exactly x: zero operands, so that the sums are the bias."""
+    n = x.numel()
+    a, sa = K().quantize_blocks(torch.zeros(m, 1024, device=DEV))
+    w, sw = K().quantize_weight_blocks(torch.ones(n, 1024, device=DEV))
+    return K().gemm_fp8(a, sa, w, sw, x, act=K().ACT_GELU, out_dtype=dtype)
+
+
+def between(points, a):
+    """The exponential of the straight line between the points' logarithms, at a."""
+    at, val = (torch.tensor(v, dtype=torch.float64, device=a.device) for v in zip(*points))
+    i = torch.bucketize(a, at).clamp(1, len(points) - 1)
+    f = ((a - at[i - 1]) / (at[i] - at[i - 1])).clamp(0, 1)
+    return torch.exp(val[i - 1].log() * (1 - f) + val[i].log() * f)
+
+
+def gelu_ref(x, fit):
+    """GELU(x) in 64 bits and the bound of its error.
+
+    GELU(x) = max(x, 0) - t with t = a Phi(-a), a = |x|, and Phi(-a) = 2^q with
+    a polynomial q.  `fit` bounds what the polynomial, with its fp32
+    coefficients, is off, relative to Phi.  Horner's scheme rounds the partial
+    sum p_k, which is still to be multiplied by a^k, by at most U32 |p_k|: in q
+    that is U32 HORNER(a), in Phi ln 2 times as much.  2^q is off by 2^-22 at
+    most, the last product and the sum by a rounding each.  Beyond 12.9, where
+    t is below 4e-37, it may be dropped."""
+    x = x.double()
+    a = x.abs()
+    t = a * 0.5 * torch.erfc(a / math.sqrt(2.0))
+    rel = between(fit, a) + U32 * (4 + 1 + math.log(2.0) * between(HORNER, a))
+    ref = x.clamp_min(0) - t
+    return ref, t * rel + U32 * ref.abs() + torch.where(a > 12.9, 4e-37, 0.0)
+
+
+# sum_k |p_k| a^k: 1, 4.87, 12.6, 25, 58.7, 147, 704, 3890, 19100 and 49200 at
+# these points for degree 13, less for degree 7; a straight line between their
+# logarithms falls below it by 14 % at most.
+HORNER = [(0, 1.2), (1, 5.7), (2, 14.5), (3, 29), (4.5, 68), (6, 170), (8, 815), (10, 4500),
+          (12, 22100), (13.3, 57000)]
+# Largest difference between the neighbouring points.
+FIT32 = [(0, 1.8e-8), (0.5, 1.8e-8), (1, 2.9e-8), (1.5, 2.9e-8), (2, 1.9e-7), (2.5, 3.2e-7),
+         (3, 1.6e-6), (3.5, 1.7e-6), (4, 2e-5), (5, 3.2e-5), (6, 6.3e-5), (8, 1.3e-4),
+         (10, 2.9e-4), (13.3, 2.9e-4)]
+FIT16 = [(0, 8.7e-7), (0.25, 1.9e-6), (0.5, 1.9e-6), (1, 2.5e-6), (1.5, 3e-6), (2, 1.4e-5),
+         (2.5, 1.5e-5), (3, 1.4e-4), (3.5, 3.9e-4), (4, 8.2e-4), (5, 8.2e-4), (6, 0.011),
+         (8, 0.012), (10, 0.1), (13.3, 0.1)]
+
+
+def gelu_inputs(g, n):
+    """Values over the whole range: tiny, ordinary, in the tail and beyond it."""
+    x = torch.exp(torch.empty(n, device=DEV).uniform_(math.log(1e-6), math.log(20.0), generator=g))
+    x[n // 2:] = torch.empty(n - n // 2, device=DEV).uniform_(0, 14, generator=g)
+    x = x * torch.where(torch.rand(n, device=DEV, generator=g) < 0.7, -1.0, 1.0)
+    x[:6] = torch.tensor([0.0, -100.0, 100.0, -1e30, 1e30, -13.0], device=DEV)
+    return x
+
+
+@pytest.mark.parametrize("m", GELU_ROWS)
+def test_gelu_fp32(m):
+    """To a few roundings of the result near zero, and right in the tail."""
+    x = gelu_inputs(gen(m, 31), 4096)
+    ref, tol = gelu_ref(x, FIT32)
+    near = (x.abs() <= 1) & (x != 0)
+    assert (tol[near] <= 14 * U32 * ref[near].abs()).all()  # what the bound above comes to
+    out = gelu_of(x, m, torch.float32).double()
+    bad = (out - ref).abs() > tol
+    assert not bad.any(), x.expand_as(out)[bad][:8]
+
+
+@pytest.mark.parametrize("m", GELU_ROWS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gelu_16_bit(m, dtype):
+    x = gelu_inputs(gen(m, 32), 4096).clamp(-60000, 60000)
+    ref, tol = gelu_ref(x, FIT16)
+    check_out(gelu_of(x, m, dtype), ref.expand(m, -1), tol)
+
+
+@pytest.mark.parametrize("m", GELU_ROWS)
+def test_gelu_blocks_of_the_tail(m):
+    """Blocks of small results only: their 8-bit values keep the results' ratios."""
+    g = gen(m, 33)
+    lo = torch.tensor([-1e-4, -2.0, -5.0, -7.0, -9.0, -12.0, -40.0], device=DEV)
+    x = (lo[:, None] * (1 + 0.1 * torch.rand(7, 128, device=DEV, generator=g))).flatten()
+    ref, tol = gelu_ref(x, FIT16)
+    q, s = gelu_of(x, m, F8)
+    check_quantised(q, s, ref.expand(m, -1).contiguous(), tol)
+    assert (q[:, -128:].float() == 0).all()
+
+
+@pytest.mark.parametrize("m", GELU_ROWS)
+def test_gelu_of_infinities(m):
+    """As 0.5 x (1 + erf(x / sqrt 2)): NaN at minus infinity, infinity at infinity."""
+    x = rand(gen(m, 34), 512)
+    x[5], x[200], x[300] = -math.inf, math.inf, math.nan
+    for dtype in DTYPES:
+        out = gelu_of(x, m, dtype)
+        assert out[:, 5].isnan().all() and (out[:, 200] == math.inf).all()
+        assert out[:, 300].isnan().all()
+        rest = torch.ones(512, dtype=torch.bool, device=DEV)
+        rest[[5, 200, 300]] = False
+        assert out[:, rest].isfinite().all()
+    q, s = gelu_of(x, m, F8)
+    held = q.double() * per_block(s, m, 512)
+    assert held[:, :384].isnan().all() and held[:, 384:].isfinite().all()
+
+
+@pytest.mark.parametrize("m", [5, 90, 600, 9000])
+def test_infinite_scale_under_gelu(m):
+    """A row whose scale is infinite ends with no finite value."""
+    g = gen(m, 35)
+    a, sa, w, sw = operands(g, m, 768, 528)
+    sa[m - 1, 2] = math.inf
+    for dtype in DTYPES:
+        out = K().gemm_fp8(a, sa, w, sw, act=K().ACT_GELU, out_dtype=dtype)
+        assert not out[m - 1].isfinite().any() and out[:m - 1].isfinite().all()

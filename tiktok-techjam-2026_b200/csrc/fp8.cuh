@@ -101,6 +101,16 @@ __device__ __forceinline__ uint32_t quantize4(float4 v, float s, float inv) {
   return quantize4(f, s, inv);
 }
 
+// log2 Phi(b) of two values b <= 0, as -1 + c[0] b + c[1] b^2 + ...
+template <int N>
+__device__ __forceinline__ void log2_phi(float& q0, float& q1, float b0, float b1,
+                                         const float (&c)[N]) {
+  q0 = q1 = c[N - 1];
+#pragma unroll
+  for (int i = N - 2; i >= 0; --i) fma2v(q0, q1, q0, q1, b0, b1, c[i], c[i]);
+  fma2v(q0, q1, q0, q1, b0, b1, -1.f, -1.f);
+}
+
 // max(x, 0), a NaN stays one.
 __device__ __forceinline__ float relu_nan(float x) {
   float r;
@@ -108,28 +118,38 @@ __device__ __forceinline__ float relu_nan(float x) {
   return r;
 }
 
-// Erf GELU of two values in seven issue slots and one MUFU operation each
-// (gelu_erf in common.cuh: eighteen and two; with one or two warps a
-// sub-partition an activation of 128 values a thread is bound by them):
-//   GELU(x) = max(x, 0) - a Phi(-a), a = |x|,
-// with log2 Phi(-a) by a polynomial of degree seven on [0, 6], fitted by
-// Lawson's iteration (weighted least squares towards the minimax) to the
-// error of a Phi(-a): 2.5e-7 absolute in fp32, and 6e-5 relative in the
-// negative tail.  Beyond 6 the tail stays at its -6e-9.  A NaN comes through
-// the maximum.
+// Erf GELU of two values, packed (gelu_erf in common.cuh takes twice the issue
+// slots and two MUFU operations a value; with one or two warps a sub-partition
+// an activation of 128 values a thread is bound by them):
+//   GELU(x) = max(x, 0) + b Phi(b), b = -|x|,
+// with log2 Phi(b) by a polynomial on [-13.3, 0], where 2^q leaves fp32's
+// normal range and becomes zero.  Both are fitted by Lawson's iteration
+// (weighted least squares towards the minimax) with Phi(0) = 1/2 exactly.
+// kFine, for fp32 results, degree 13: Phi(b) to 3e-8 of itself down to -2,
+// 2e-5 to -5 and 3e-4 to the end, before the roundings in fp32 (2e-7, 3e-6 and
+// up to 2e-3) and of 2^q (2^-22): for |x| <= 1 the GELU is within 12 x 2^-24 of
+// itself.
+// Else, for results that are rounded to 16 or 8 bits (by 2e-4 of themselves or
+// more), degree 7: the GELU to 3e-7 absolute, 3e-6 of itself for |x| <= 2, 8e-4
+// to -5.5, 0.012 to -9 and a tenth to the end.
+// The factor of a negative x is not cut at 13.3: minus infinity times zero is
+// NaN, as in 0.5 x (1 + erf(x / sqrt 2)).
+template <bool kFine>
 __device__ __forceinline__ void gelu_pair(float& x0, float& x1) {
-  const float a0 = fminf(fabsf(x0), 6.f), a1 = fminf(fabsf(x1), 6.f);
+  const float b0 = fmaxf(-fabsf(x0), -13.3f), b1 = fmaxf(-fabsf(x1), -13.3f);
   float q0, q1, e0, e1;
-  fma2v(q0, q1, a0, a1, -1.43977059e-06f, -1.43977059e-06f, 5.48538883e-05f, 5.48538883e-05f);
-  fma2v(q0, q1, q0, q1, a0, a1, -0.000887982082f, -0.000887982082f);
-  fma2v(q0, q1, q0, q1, a0, a1, 0.00838699006f, 0.00838699006f);
-  fma2v(q0, q1, q0, q1, a0, a1, -0.0538126267f, -0.0538126267f);
-  fma2v(q0, q1, q0, q1, a0, a1, -0.458510876f, -0.458510876f);
-  fma2v(q0, q1, q0, q1, a0, a1, -1.15127623f, -1.15127623f);
-  fma2v(q0, q1, q0, q1, a0, a1, -0.999986351f, -0.999986351f);
+  if constexpr (kFine)
+    log2_phi(q0, q1, b0, b1,
+             {1.15110481f, -0.459216624f, 0.0524468757f, 0.00693850731f, -2.76900973e-05f,
+              -0.000308792718f, -9.25991262e-05f, -1.62199449e-05f, -1.88740239e-06f,
+              -1.47035465e-07f, -7.36164862e-09f, -2.13845219e-10f, -2.73576496e-12f});
+  else
+    log2_phi(q0, q1, b0, b1,
+             {1.15114117f, -0.458884239f, 0.0533754863f, 0.00814140774f, 0.000821109221f,
+              4.67876635e-05f, 1.11061843e-06f});
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(q0));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(q1));
-  fma2v(x0, x1, -a0, -a1, e0, e1, relu_nan(x0), relu_nan(x1));
+  fma2v(x0, x1, fminf(b0, x0), fminf(b1, x1), e0, e1, relu_nan(x0), relu_nan(x1));
 }
 
 // Four consecutive elements of a row: raw as loaded (16 or 8 bytes), widened

@@ -158,8 +158,13 @@ __device__ __forceinline__ void finish4(const GemmF8Args& args, float4 v, float4
   v.z += bias.z;
   v.w += bias.w;
   if (args.act == 1) {
-    gelu_pair(v.x, v.y);
-    gelu_pair(v.z, v.w);
+    if (args.out_dtype == TJB_F32) {
+      gelu_pair<true>(v.x, v.y);
+      gelu_pair<true>(v.z, v.w);
+    } else {
+      gelu_pair<false>(v.x, v.y);
+      gelu_pair<false>(v.z, v.w);
+    }
   }
   if (args.out_dtype == TJB_E4M3) {
     if (n >= args.N) v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -953,8 +958,13 @@ __global__ void __launch_bounds__(WideCfg<kForm>::kThreads, 1)
       if (!ok) break;
       if (n0 >= args.N || !has) continue;  // warp-uniform
       if (args.act == 1) {
+        if (args.out_dtype == TJB_F32) {
 #pragma unroll
-        for (int j = 0; j < 128; j += 2) gelu_pair(sum[j], sum[j + 1]);
+          for (int j = 0; j < 128; j += 2) gelu_pair<true>(sum[j], sum[j + 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 128; j += 2) gelu_pair<false>(sum[j], sum[j + 1]);
+        }
       }
       const int row0 = m_blk * 128 + quad * 32;
       // Up to two 32-row x 128-byte pieces of this warp at a time: wait until
