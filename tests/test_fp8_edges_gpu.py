@@ -182,3 +182,41 @@ def test_infinite_scale_under_gelu(m):
     for dtype in DTYPES:
         out = K().gemm_fp8(a, sa, w, sw, act=K().ACT_GELU, out_dtype=dtype)
         assert not out[m - 1].isfinite().any() and out[:m - 1].isfinite().all()
+
+
+# ------------------------------------------------------------- infinite blocks
+
+def e4m3_of(y, s):
+    """e4m3(y / s), with what inf / inf and finite / inf are."""
+    return (y.double() / s).float().to(F8)
+
+
+def test_bytes_of_infinite_blocks():
+    """q = e4m3(y / s) also where s is infinite or NaN: zeros beside the NaN of
+    an infinite element, NaN throughout a block with a NaN."""
+    x = rand(gen(36), 8, 512) * 3
+    x[0, 3], x[1, 130], x[2, 200] = math.inf, -math.inf, math.nan
+    x[3, 300], x[3, 301] = math.inf, math.nan
+    x[4] = math.inf
+    want_s = x.abs().view(8, 4, 128).amax(dim=2)
+    for dtype in DTYPES:
+        y = x.to(dtype)
+        q, s = K().quantize_blocks(y)
+        odd = per_block(want_s, 8, 512).isfinite().logical_not()
+        want = e4m3_of(y, per_block(want_s, 8, 512))
+        got, want = q.float()[odd], want.float()[odd]
+        assert torch.equal(got.isnan(), want.isnan()) and (got[~got.isnan()] == 0).all()
+        assert got.isnan().any() and (~got.isnan()).any()
+        qw, sw = K().quantize_weight_blocks(y[:1])
+        assert sw[0, 0].isinf() and qw[0, 3].isnan() and (qw[0, :3].float() == 0).all()
+    # As an output of the norm (an infinite weight) and of the product (a bias).
+    w = torch.ones(512, device=DEV)
+    w[7] = math.inf
+    q, s = K().rmsnorm(x[5:7], w, 1e-5, out_dtype=F8)
+    assert s[:, 0].isinf().all() and q[:, 7].isnan().all() and (q[:, 8:128].float() == 0).all()
+    for m in (3, 100, 9000):
+        a, sa, wq, ws = operands(gen(m, 37), m, 512, 256)
+        bias = torch.zeros(512, device=DEV)
+        bias[7] = math.inf
+        q, s = K().gemm_fp8(a, sa, wq, ws, bias, out_dtype=F8)
+        assert s[:, 0].isinf().all() and q[:, 7].isnan().all() and (q[:, 8:128].float() == 0).all()

@@ -52,15 +52,14 @@ __device__ __forceinline__ float warp_max_abs(float v) {
 // its remainder (Markstein, IBM J. Res. Dev. 34, 1990).  The plain product
 // v * inv moves about one value in 10^6 across a rounding border of the 8-bit
 // type, and full divisions bound the memory-bound kernels here by their
-// instructions (a 65536 x 4096 norm: 540 us against 461).  With s NaN or
-// infinite: NaN.
+// instructions (a 65536 x 4096 norm: 540 us against 461).
 __device__ __forceinline__ float div_by(float v, float s, float inv) {
   const float q = v * inv;
   return fmaf(fmaf(-q, s, v), inv, q);
 }
 
-// 1 / s for s in [2^-126, 2^126): the hardware's approximation and one step
-// of Newton's iteration.
+// 1 / s for s in [2^-126, 2^126]: the hardware's approximation and one step
+// of Newton's iteration.  Larger s give zero.
 __device__ __forceinline__ float reciprocal(float s) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
@@ -74,8 +73,21 @@ __device__ __forceinline__ float block_scale(float amax) {
   return fmaxf(s, 1.17549435e-38f);
 }
 
-// Four e4m3 bytes of v / s, the first in the lowest byte (inv = 1 / s).
-__device__ __forceinline__ uint32_t quantize4(const float* v, float s, float inv) {
+// A scale as quantize4 divides by it: s and 1 / s.  An infinite s becomes the
+// largest number, whose reciprocal underflows to zero here: finite values give
+// zero and infinite ones NaN, as finite / inf and inf / inf do.  A NaN stays.
+struct Divisor {
+  float s, inv;
+};
+__device__ __forceinline__ Divisor divisor(float s) {
+  Divisor d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d.s) : "f"(s), "f"(3.40282347e38f));
+  d.inv = reciprocal(d.s);
+  return d;
+}
+
+// Four e4m3 bytes of v / d.s, the first in the lowest byte.
+__device__ __forceinline__ uint32_t quantize4(const float* v, Divisor d) {
   float q[4], e[4];
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {  // div_by on packed pairs
@@ -85,9 +97,9 @@ __device__ __forceinline__ uint32_t quantize4(const float* v, float s, float inv
         "mul.rn.f32x2 ra, ra, rb;\n\t"
         "mov.b64 {%0, %1}, ra;\n\t}"
         : "=f"(q[i]), "=f"(q[i + 1])
-        : "f"(v[i]), "f"(v[i + 1]), "f"(inv));
-    fma2v(e[i], e[i + 1], q[i], q[i + 1], -s, -s, v[i], v[i + 1]);
-    fma2v(q[i], q[i + 1], e[i], e[i + 1], inv, inv, q[i], q[i + 1]);
+        : "f"(v[i]), "f"(v[i + 1]), "f"(d.inv));
+    fma2v(e[i], e[i + 1], q[i], q[i + 1], -d.s, -d.s, v[i], v[i + 1]);
+    fma2v(q[i], q[i + 1], e[i], e[i + 1], d.inv, d.inv, q[i], q[i + 1]);
   }
   const __nv_fp8x2_storage_t lo =
       __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
@@ -96,9 +108,9 @@ __device__ __forceinline__ uint32_t quantize4(const float* v, float s, float inv
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 
-__device__ __forceinline__ uint32_t quantize4(float4 v, float s, float inv) {
+__device__ __forceinline__ uint32_t quantize4(float4 v, Divisor d) {
   const float f[4] = {v.x, v.y, v.z, v.w};
-  return quantize4(f, s, inv);
+  return quantize4(f, d);
 }
 
 // log2 Phi(b) of two values b <= 0, as -1 + c[0] b + c[1] b^2 + ...

@@ -171,7 +171,7 @@ __device__ __forceinline__ void finish4(const GemmF8Args& args, float4 v, float4
     const float s = block_scale(warp_max_abs(max_abs4(v)));
     if (n < args.N)
       *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(args.C) + m * args.ldc + n) =
-          quantize4(v, s, reciprocal(s));
+          quantize4(v, divisor(s));
     if (lane == 0) args.c_scales[m * ((args.N + kQBlock - 1) / kQBlock) + n / kQBlock] = s;
   } else if (n < args.N) {
     store4(args.C, args.out_dtype, m * args.ldc + n, v);
@@ -992,10 +992,10 @@ __global__ void __launch_bounds__(WideCfg<kForm>::kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 128; j += 2) top = max_abs(top, sum[j], sum[j + 1]);
         const float s = block_scale(top);
-        const float inv = reciprocal(s);
+        const Divisor div = divisor(s);
         uint32_t w[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) w[j] = quantize4(&sum[4 * j], s, inv);
+        for (int j = 0; j < 32; ++j) w[j] = quantize4(&sum[4 * j], div);
         stage_row(buf, lane, w);
         out_send(1, n0, 128);
         if (row0 + lane < args.M)

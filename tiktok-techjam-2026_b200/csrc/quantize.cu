@@ -53,12 +53,12 @@ __global__ void __launch_bounds__(kQuantThreads)
       top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (col < K) {
       const float s = block_scale(__uint_as_float(top));
-      const float inv = reciprocal(s);
+      const Divisor div = divisor(s);
       float f[kElems];
       piece[i].widen(f);
       uint32_t b[kElems / 4];
 #pragma unroll
-      for (int j = 0; j < kElems / 4; ++j) b[j] = quantize4(f + 4 * j, s, inv);
+      for (int j = 0; j < kElems / 4; ++j) b[j] = quantize4(f + 4 * j, div);
       uint8_t* dst = q + row * K + col;
       if constexpr (kElems == 8)
         *reinterpret_cast<uint2*>(dst) = make_uint2(b[0], b[1]);
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kQuantThreads)
 #pragma unroll
     for (int i = 0; i < kQuantThreads / 32; ++i) top = max_abs(top, s_max[odd][i]);
     const float s = block_scale(top);
-    const float inv = reciprocal(s);
+    const Divisor div = divisor(s);
     const int nb = tile / kb_count;
     const int col = (tile - nb * kb_count) * kQBlock + c0;
 #pragma unroll
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kQuantThreads)
       piece[i].widen(f);
       uint32_t b[kElems / 4];
 #pragma unroll
-      for (int j = 0; j < kElems / 4; ++j) b[j] = quantize4(f + 4 * j, s, inv);
+      for (int j = 0; j < kElems / 4; ++j) b[j] = quantize4(f + 4 * j, div);
       if (row < N && col < K) {
         uint8_t* dst = q + static_cast<int64_t>(row) * K + col;
         if constexpr (kElems == 8)

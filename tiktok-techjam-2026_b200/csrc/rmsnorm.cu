@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
       const float s = block_scale(warp_max_abs(max_abs4(y)));
       if (col < d)
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + base + col) =
-            quantize4(y, s, reciprocal(s));
+            quantize4(y, divisor(s));
       if ((t & 31) == 0) out_scales[row * kb_count + kb] = s;
     } else if (col < d) {
       store4(out, out_dtype, base + col, y);
@@ -208,10 +208,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
       const float s = block_scale(__uint_as_float(bits));
-      const float inv = reciprocal(s);
+      const Divisor div = divisor(s);
       if (col < d) {
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(out) + base + col) =
-            make_uint2(quantize4(y, s, inv), quantize4(y + 4, s, inv));
+            make_uint2(quantize4(y, div), quantize4(y + 4, div));
         if ((t & 15) == 0) out_scales[row * kb_count + col / kQBlock] = s;
       }
     } else if (col < d) {
