@@ -444,8 +444,8 @@ int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out, void* out
  * scales whose product leaves the type's normal range lose what it cannot
  * hold.  A call's result depends on nothing but its operands (no atomics, no
  * workspace).  K % 16 == 0, N % 8 == 0 (e4m3 output: N % 16 == 0), both at
- * most 2^31 - 1025; lda and ldw multiples of 16, ldc of 8 (e4m3:
- * 16); 16-byte aligned A, W, C and bias.  m_tiles (nullable) as in
+ * most 2^31 - 1025; lda, ldw and ldc multiples of 16 bytes; 16-byte aligned A,
+ * W, C and bias.  m_tiles (nullable) as in
  * tjb_row_tiles.
  * The 8-bit sibling of tjb_gemm_bias; no counterpart in the reference.
  */

@@ -220,3 +220,22 @@ def test_bytes_of_infinite_blocks():
         bias[7] = math.inf
         q, s = K().gemm_fp8(a, sa, wq, ws, bias, out_dtype=F8)
         assert s[:, 0].isinf().all() and q[:, 7].isnan().all() and (q[:, 8:128].float() == 0).all()
+
+
+# ------------------------------------------------------------------ the output
+
+@pytest.mark.parametrize("m", [5, 40, 100, 700, 11000])
+def test_fp32_rows_at_any_16_byte_pitch(m):
+    g = gen(m, 38)
+    n, k = 520, 656
+    a, sa, w, sw = operands(g, m, n, k)
+    out = torch.full((m, n + 12), 7.0, device=DEV)
+    got = K().gemm_fp8(a, sa, w, sw, out_dtype=torch.float32, out=out[:, :n])
+    assert got.data_ptr() == out.data_ptr()
+    assert torch.equal(out[:, :n], K().gemm_fp8(a, sa, w, sw, out_dtype=torch.float32))
+    assert (out[:, n:] == 7).all()
+    from tjkernels._lib import KernelError
+    if m > 1:
+        with pytest.raises(KernelError):
+            K().gemm_fp8(a, sa, w, sw, out_dtype=torch.float16,
+                         out=torch.zeros(m, n + 4, device=DEV, dtype=torch.float16)[:, :n])

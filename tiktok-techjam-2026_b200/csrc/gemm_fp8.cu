@@ -1167,12 +1167,13 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
   if (act != 0 && act != 1) return TJB_ERR_INVALID_ARGUMENT;
   const bool q = out_dtype == TJB_E4M3;
   if (q && !c_scales) return TJB_ERR_INVALID_ARGUMENT;
-  const int unit = q ? 16 : 8;  // output columns: whole 16-byte pieces
+  const int unit = q ? 16 : 8;  // output columns
+  const int pitch = out_dtype == TJB_F32 ? 4 : unit;  // 16 bytes
   if (K % 16 != 0 || N % unit != 0 || K > kMaxColumns || N > kMaxColumns || lda < K || ldw < K ||
       ldc < N || M > 2147483647 - kLiveTileRows)
     return TJB_ERR_BAD_SHAPE;
   auto misaligned4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; };
-  if (lda % 16 != 0 || ldw % 16 != 0 || ldc % unit != 0 || !aligned16(A) || !aligned16(W) ||
+  if (lda % 16 != 0 || ldw % 16 != 0 || ldc % pitch != 0 || !aligned16(A) || !aligned16(W) ||
       !aligned16(C) || (bias && !aligned16(bias)) || misaligned4(a_scales) ||
       misaligned4(w_scales) || (q && misaligned4(c_scales)))
     return TJB_ERR_BAD_ALIGNMENT;
