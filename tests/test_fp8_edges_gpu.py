@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_fp8_gpu import (DEV, F8, NORM_REL, U32, K, check_out, check_quantised, gen, operands,
-                          per_block, rand, rms_ref)
+                          per_block, product_ref, rand, rms_ref)
 
 pytestmark = pytest.mark.gpu
 
@@ -239,3 +239,22 @@ def test_fp32_rows_at_any_16_byte_pitch(m):
         with pytest.raises(KernelError):
             K().gemm_fp8(a, sa, w, sw, out_dtype=torch.float16,
                          out=torch.zeros(m, n + 4, device=DEV, dtype=torch.float16)[:, :n])
+
+
+def test_as_many_rows_as_an_int_counts():
+    """The most tokens of a call: counts of them, rounded up to tiles of 256."""
+    m, n, k = 2 ** 31 - 129, 8, 16
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 90e9:
+        pytest.skip("needs 70 GB of device memory")
+    g = gen(39)
+    tail, sa, w, sw = operands(g, 500, n, k)
+    a = torch.zeros(m, k, dtype=torch.uint8, device=DEV)
+    a[-500:] = tail.view(torch.uint8)
+    out = torch.full((m, n), 7.0, dtype=torch.float16, device=DEV)
+    K().gemm_fp8(a.view(F8), sa[:1].expand(m, 1), w, sw, out_dtype=torch.float16, out=out)
+    ref, tol = product_ref(tail, sa[:1].expand(500, 1), w, sw)
+    check_out(out[-500:], ref, tol)
+    assert (out[:4096] == 0).all() and (out[:-500:65537] == 0).all()
+    del a, out
+    torch.cuda.empty_cache()

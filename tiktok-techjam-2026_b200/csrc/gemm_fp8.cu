@@ -1122,7 +1122,8 @@ int launch_wide(const void* A, const void* W, GemmF8Args args, int lda, int ldw,
   const int wide_n = (args.N + 255) / 256;
   args.splits = 1;
   if (pairs > 0) {
-    const int tiles = (args.M + 255) / 256 * wide_n;
+    // (64 bits: M comes within 129 of 2^31.)
+    const int tiles = static_cast<int>((args.M + INT64_C(255)) / 256) * wide_n;
     args.first_tile = 0;
     args.end_tile = tiles;
     return launch_kernel_cluster(gemm_fp8_wide_kernel<kPaired>,
