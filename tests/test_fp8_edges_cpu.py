@@ -10,9 +10,7 @@ from test_fp8_cpu import gemm
 @pytest.mark.parametrize("out,pitch", [(0, 4), (1, 8), (2, 8), (3, 16)])
 def test_output_rows_start_on_16_byte_borders(out, pitch):
     """Any such pitch is taken, whatever the type; no other is."""
-    for n in range(1, 16):
-        got = gemm(n=256, ldc=256 + n, out=out)
-        if n % pitch:
-            assert got == 3, n
-        elif not torch.cuda.is_available():
-            assert got == 8, n
+    if torch.cuda.is_available():
+        pytest.skip("the made-up addresses are for machines without a GPU")
+    for n in range(1, 17):
+        assert gemm(n=256, ldc=256 + n, out=out) == (3 if n % pitch else 8), n
