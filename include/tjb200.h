@@ -418,7 +418,8 @@ int tjb_quantize_weight_blocks(const void* w, int64_t ldw, int in_dtype, void* q
  * The norm reads the unrounded sum.  res, res_out: res_dtype; delta:
  * delta_dtype (each f32, f16 or bf16); w: fp32 [d]; out: f32, f16, bf16, or
  * TJB_E4M3 with out_scales [rows, ceil(d/128)] (see tjb_quantize_blocks;
- * ignored otherwise).  All contiguous; res_out may alias res.  d <= 16384,
+ * ignored otherwise).  All contiguous; res_out may be res, or a delta of its
+ * type, and overlaps no operand otherwise.  d <= 16384,
  * d % 4 == 0 (e4m3: d % 16 == 0).  row_mask (nullable): rows with 0 get a
  * zero output row; m_tiles (nullable) as in tjb_row_tiles.
  * The 8-bit-capable RMS sibling of fused_add_layernorm
@@ -445,7 +446,7 @@ int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out, void* out
  * hold.  A call's result depends on nothing but its operands (no atomics, no
  * workspace).  K % 16 == 0, N % 8 == 0 (e4m3 output: N % 16 == 0), both at
  * most 2^31 - 1025; lda, ldw and ldc multiples of 16 bytes; 16-byte aligned A,
- * W, C and bias.  m_tiles (nullable) as in
+ * W, C and bias; C and c_scales overlap no operand.  m_tiles (nullable) as in
  * tjb_row_tiles.
  * The 8-bit sibling of tjb_gemm_bias; no counterpart in the reference.
  */

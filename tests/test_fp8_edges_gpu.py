@@ -258,3 +258,31 @@ def test_as_many_rows_as_an_int_counts():
     assert (out[:4096] == 0).all() and (out[:-500:65537] == 0).all()
     del a, out
     torch.cuda.empty_cache()
+
+
+def test_outputs_over_an_operand_are_refused():
+    """While a call writes its output other blocks of it still read the operands."""
+    g = gen(40)
+    a, sa, w, sw = operands(g, 300, 256, 256)
+    for out in (a, a[:200], w):
+        with pytest.raises(ValueError):
+            K().gemm_fp8(a[:out.shape[0]], sa[:out.shape[0]], w, sw, out_dtype=F8, out=out)
+    both = torch.zeros(300, 512, device=DEV).to(F8)
+    both[:, :256] = a
+    want, scales = K().gemm_fp8(a, sa, w, sw, out_dtype=F8)
+    got, s = K().gemm_fp8(both[:, :256], sa, w, sw, out_dtype=F8, out=both[:, 256:])
+    assert torch.equal(got.float(), want.float()) and torch.equal(s, scales)
+    assert torch.equal(both[:, :256].float(), a.float())
+    nw = torch.ones(256, device=DEV)
+    buf = rand(g, 101, 256).half()
+    with pytest.raises(ValueError):
+        K().fused_add_rmsnorm(buf[1:], rand(g, 100, 256), nw, 1e-5, residual_out=buf[:-1])
+    with pytest.raises(ValueError):
+        K().fused_add_rmsnorm(rand(g, 100, 256).half(), buf[1:], nw, 1e-5, residual_out=buf[:-1])
+    with pytest.raises(ValueError):  # the same address, another type
+        K().fused_add_rmsnorm(buf[:100], buf.view(torch.bfloat16)[:100], nw, 1e-5,
+                              residual_out=buf[:100])
+    res, delta = rand(g, 100, 256).half(), rand(g, 100, 256).half()
+    want, out = K().fused_add_rmsnorm(res, delta, nw, 1e-5)
+    got, out2 = K().fused_add_rmsnorm(res, delta, nw, 1e-5, residual_out=delta)
+    assert got is delta and torch.equal(delta, want) and torch.equal(out2, out)

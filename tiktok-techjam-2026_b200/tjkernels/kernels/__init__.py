@@ -490,6 +490,27 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, pitch
 
 
+def _need_apart(what: str, out: torch.Tensor, *inputs: Optional[torch.Tensor]) -> None:
+    """``out`` shares no element with any of ``inputs`` (matrices of
+    consecutive columns, or None): other threads of the call still read them
+    while it is written."""
+    def span(t):
+        size = t.element_size()
+        return t.data_ptr(), t.stride(0) * size, t.shape[1] * size, t.shape[0]
+
+    at, pitch, row, rows = span(out)
+    for t in inputs:
+        if t is None or t.numel() == 0 or out.numel() == 0:
+            continue
+        at2, pitch2, row2, rows2 = span(t)
+        if at2 >= at + (rows - 1) * pitch + row or at >= at2 + (rows2 - 1) * pitch2 + row2:
+            continue
+        # Interleaved columns of one buffer: the rows of one lie in the other's gaps.
+        gap = (at2 - at) % pitch if pitch == pitch2 and pitch else 0
+        if gap < row or gap + row2 > pitch:
+            raise ValueError(f"{what} overlaps an operand of the call")
+
+
 def _check_tiles(m_tiles: torch.Tensor, device: torch.device, rows: int) -> int:
     _same_device(device, m_tiles)
     if m_tiles.dtype != torch.int32 or not m_tiles.is_contiguous() \
@@ -568,7 +589,8 @@ def fused_add_rmsnorm(
     norm (d a multiple of 16; otherwise of 4; at most 16384).
     ``write_residual``, ``residual_out`` (may be ``residual``), ``row_mask``
     and ``m_tiles`` as in :func:`fused_add_layernorm`; a ``residual_out`` that
-    is given without a ``delta`` receives ``residual``."""
+    is given without a ``delta`` receives ``residual``, and one that overlaps
+    an operand otherwise than as the whole of it is refused."""
     device = residual.device
     _same_device(device, delta, weight)
     if residual.dim() != 2 or not residual.is_contiguous():
@@ -614,6 +636,10 @@ def fused_add_rmsnorm(
         if residual_out.shape != shape or residual_out.dtype != dtype \
                 or not residual_out.is_contiguous():
             raise ValueError("residual_out must be contiguous, of residual's shape and dtype")
+        # (The same elements of the same type are read before they are written.)
+        _need_apart("residual_out", residual_out,
+                    *(t for t in (residual, delta) if t is not None
+                      and (t.data_ptr() != residual_out.data_ptr() or t.dtype != dtype)))
         new = residual_out
         new_at = new.data_ptr()
     elif write_residual and delta is not None:
@@ -643,8 +669,8 @@ def gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales:
     bf16, or float8_e4m3fn, which returns ``(q, scales)`` as
     :func:`quantize_blocks` of the fp32 result would.  K must be a multiple of
     16, N of 8 (e4m3 output: 16).  ``out``: a [M, N] tensor of ``out_dtype`` to
-    write (rows at any 16-byte pitch).  With ``m_tiles`` only the listed
-    128-row tiles are computed."""
+    write (rows at any 16-byte pitch), which no operand overlaps.  With
+    ``m_tiles`` only the listed 128-row tiles are computed."""
     device = a.device
     _same_device(device, a_scales, w, w_scales, bias, out)
     if a.dim() != 2 or w.dim() != 2:
@@ -683,6 +709,7 @@ def gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales:
     else:
         if out.shape != (m, n) or out.dtype != out_dtype or (m and n > 1 and out.stride(1) != 1):
             raise ValueError("out must be an [M, N] tensor of out_dtype with consecutive columns")
+        _need_apart("out", out, a, w)
         if m > 1:
             ldc = out.stride(0)
             if ldc > _INT_MAX:
