@@ -440,8 +440,9 @@ int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out, void* out
  * [N] or NULL; act: 0 = none, 1 = erf GELU, to 12 x 2^-24 of itself for sums
  * up to 1 in magnitude and to 5e-7 beyond with C in f32, to 5e-7 with the
  * other types (before C's rounding); NaN at minus infinity, as
- * 0.5 x (1 + erf(x / sqrt 2)).  C (rows ldc elements apart): f32, f16, bf16,
- * or TJB_E4M3 with c_scales contiguous [M, ceil(N/128)].  fp32 accumulation; sa * sw is one fp32 product, so
+ * 0.5 x (1 + erf(x / sqrt 2)), and for TJB_E4M3 at plus infinity too.  C (rows
+ * ldc elements apart): f32, f16, bf16, or TJB_E4M3 with c_scales contiguous
+ * [M, ceil(N/128)].  fp32 accumulation; sa * sw is one fp32 product, so
  * scales whose product leaves the type's normal range lose what it cannot
  * hold.  A call's result depends on nothing but its operands (no atomics, no
  * workspace).  K % 16 == 0, N % 8 == 0 (e4m3 output: N % 16 == 0), both at

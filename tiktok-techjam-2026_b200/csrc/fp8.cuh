@@ -137,20 +137,23 @@ __device__ __forceinline__ float relu_nan(float x) {
 // with log2 Phi(b) by a polynomial on [-13.3, 0], where 2^q leaves fp32's
 // normal range and becomes zero.  Both are fitted by Lawson's iteration
 // (weighted least squares towards the minimax) with Phi(0) = 1/2 exactly.
-// kFine, for fp32 results, degree 13: Phi(b) to 3e-8 of itself down to -2,
-// 2e-5 to -5 and 3e-4 to the end, before the roundings in fp32 (2e-7, 3e-6 and
-// up to 2e-3) and of 2^q (2^-22): for |x| <= 1 the GELU is within 12 x 2^-24 of
-// itself.
-// Else, for results that are rounded to 16 or 8 bits (by 2e-4 of themselves or
-// more), degree 7: the GELU to 3e-7 absolute, 3e-6 of itself for |x| <= 2, 8e-4
-// to -5.5, 0.012 to -9 and a tenth to the end.
-// The factor of a negative x is not cut at 13.3: minus infinity times zero is
-// NaN, as in 0.5 x (1 + erf(x / sqrt 2)).
-template <bool kFine>
+// 32-bit results, degree 13: Phi(b) to 3e-8 of itself down to -2, 2e-5 to -5
+// and 3e-4 to the end, before the roundings in fp32 (2e-7, 3e-6 and up to 2e-3)
+// and of 2^q (2^-22): for |x| <= 1 the GELU is within 12 x 2^-24 of itself.
+// 16 and 8 bits (a rounding of 2e-4 or more), degree 7: the GELU to 3e-7
+// absolute, 3e-6 of itself for |x| <= 2, 8e-4 to -5.5, 0.012 to -9 and a tenth
+// to the end.
+// Infinities: the factor of a negative x is not cut, and minus infinity times
+// zero is NaN, as in 0.5 x (1 + erf(x / sqrt 2)); plus infinity stays.  For 8
+// bits b is not cut either (this polynomial falls for good), which spares two
+// instructions a value (M16384 N4096 K1024, e4m3: 103 us against 108): both
+// infinities give NaN, and either way every value of the block stands for NaN.
+template <int kBits>
 __device__ __forceinline__ void gelu_pair(float& x0, float& x1) {
-  const float b0 = fmaxf(-fabsf(x0), -13.3f), b1 = fmaxf(-fabsf(x1), -13.3f);
+  const float b0 = kBits == 8 ? -fabsf(x0) : fmaxf(-fabsf(x0), -13.3f);
+  const float b1 = kBits == 8 ? -fabsf(x1) : fmaxf(-fabsf(x1), -13.3f);
   float q0, q1, e0, e1;
-  if constexpr (kFine)
+  if constexpr (kBits == 32)
     log2_phi(q0, q1, b0, b1,
              {1.15110481f, -0.459216624f, 0.0524468757f, 0.00693850731f, -2.76900973e-05f,
               -0.000308792718f, -9.25991262e-05f, -1.62199449e-05f, -1.88740239e-06f,
@@ -161,7 +164,8 @@ __device__ __forceinline__ void gelu_pair(float& x0, float& x1) {
               4.67876635e-05f, 1.11061843e-06f});
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(q0));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(q1));
-  fma2v(x0, x1, fminf(b0, x0), fminf(b1, x1), e0, e1, relu_nan(x0), relu_nan(x1));
+  const float n0 = kBits == 8 ? b0 : fminf(b0, x0), n1 = kBits == 8 ? b1 : fminf(b1, x1);
+  fma2v(x0, x1, n0, n1, e0, e1, relu_nan(x0), relu_nan(x1));
 }
 
 // Four consecutive elements of a row: raw as loaded (16 or 8 bytes), widened

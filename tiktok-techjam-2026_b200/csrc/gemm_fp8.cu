@@ -159,11 +159,14 @@ __device__ __forceinline__ void finish4(const GemmF8Args& args, float4 v, float4
   v.w += bias.w;
   if (args.act == 1) {
     if (args.out_dtype == TJB_F32) {
-      gelu_pair<true>(v.x, v.y);
-      gelu_pair<true>(v.z, v.w);
+      gelu_pair<32>(v.x, v.y);
+      gelu_pair<32>(v.z, v.w);
+    } else if (args.out_dtype == TJB_E4M3) {
+      gelu_pair<8>(v.x, v.y);
+      gelu_pair<8>(v.z, v.w);
     } else {
-      gelu_pair<false>(v.x, v.y);
-      gelu_pair<false>(v.z, v.w);
+      gelu_pair<16>(v.x, v.y);
+      gelu_pair<16>(v.z, v.w);
     }
   }
   if (args.out_dtype == TJB_E4M3) {
@@ -960,10 +963,13 @@ __global__ void __launch_bounds__(WideCfg<kForm>::kThreads, 1)
       if (args.act == 1) {
         if (args.out_dtype == TJB_F32) {
 #pragma unroll
-          for (int j = 0; j < 128; j += 2) gelu_pair<true>(sum[j], sum[j + 1]);
+          for (int j = 0; j < 128; j += 2) gelu_pair<32>(sum[j], sum[j + 1]);
+        } else if (args.out_dtype == TJB_E4M3) {
+#pragma unroll
+          for (int j = 0; j < 128; j += 2) gelu_pair<8>(sum[j], sum[j + 1]);
         } else {
 #pragma unroll
-          for (int j = 0; j < 128; j += 2) gelu_pair<false>(sum[j], sum[j + 1]);
+          for (int j = 0; j < 128; j += 2) gelu_pair<16>(sum[j], sum[j + 1]);
         }
       }
       const int row0 = m_blk * 128 + quad * 32;
