@@ -129,8 +129,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 }
 
 // The same on 16-byte pieces of eight columns, sixteen lanes to a scale block.
-// 16384 x 4096, bf16 + bf16 to 8 bits: 75 us (floor 72) against 85 in pieces of
-// four, and 79 with two chunks a thread; 8192 x 8192, bf16 alone: 51 against 69.
+// 16384 x 4096, bf16 + bf16 to 8 bits: 75 us (72 at the rate of a copy) against
+// 85 in pieces of four, and 79 with two chunks a thread; 8192 x 8192, bf16
+// alone: 51 against 69.
 template <typename T, bool kDelta, int TPR>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     add_rmsnorm16_kernel(const T* res, const T* delta, T* res_out, void* out,
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     if (col - (t & 31) * 8 >= d) break;  // warp-uniform
     float y[8] = {};
     if (col < d) {
-      if (res_out != nullptr) store8(res_out, res_dtype, base + col, v[i]);
+      if (kDelta && res_out != nullptr) store8(res_out, res_dtype, base + col, v[i]);
       if (keep) {
         const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + col));
         const float4 w1 = __ldg(reinterpret_cast<const float4*>(w + col) + 1);
@@ -249,10 +250,13 @@ extern "C" int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out
   if (rows == 0) return TJB_OK;
   if (!delta && res_out == res) res_out = nullptr;  // x is there already
   const int64_t n = m_tiles ? (rows + kLiveTileRows - 1) / kLiveTileRows * kLiveTileRows : rows;
-  // 16-byte accesses where the types and the alignment allow them.
-  const bool vec8 = res_dtype != TJB_F32 && (!delta || delta_dtype == res_dtype) && d % 8 == 0 &&
-                    aligned16(res) && (!delta || aligned16(delta)) &&
-                    (!res_out || aligned16(res_out)) && aligned16(out);
+  // 16-byte accesses where the types and the alignment allow them.  (Without a
+  // delta that kernel writes no residual: a store that hardly any call asks for
+  // cost all of them registers; 8192 x 8192 bf16 51.4 -> 53.3 us.)
+  const bool vec8 = res_dtype != TJB_F32 && d % 8 == 0 && aligned16(res) && aligned16(out) &&
+                    (delta ? delta_dtype == res_dtype && aligned16(delta) &&
+                                 (!res_out || aligned16(res_out))
+                           : !res_out);
   // Threads per row: enough for the row; with few rows, up to one chunk each,
   // since then the latency of a row counts and not the number of threads.
   const int chunk = vec8 ? 8 : 4;
