@@ -398,7 +398,7 @@ int tjb_forward_small(const tjb_small_layer* layers, int L, const float* lnf_w,
  * tjb_quantize_blocks: x [rows, K] (in_dtype f32, f16 or bf16; rows ldx
  * elements apart) -> q [rows, K] e4m3 and scales [rows, ceil(K/128)], both
  * contiguous.  K % 16 == 0, K <= 2^31 - 1025; x, its rows and q start on
- * 16-byte boundaries.
+ * 16-byte boundaries; fewer than 2^31 scales (weights: 2^30).
  * m_tiles (nullable) as in tjb_row_tiles: rows of unlisted tiles
  * are neither read nor written.
  * tjb_quantize_weight_blocks: w [N, K] (rows ldw elements apart) ->
@@ -419,8 +419,9 @@ int tjb_quantize_weight_blocks(const void* w, int64_t ldw, int in_dtype, void* q
  * delta_dtype (each f32, f16 or bf16); w: fp32 [d]; out: f32, f16, bf16, or
  * TJB_E4M3 with out_scales [rows, ceil(d/128)] (see tjb_quantize_blocks;
  * ignored otherwise).  All contiguous; res_out may be res, or a delta of its
- * type, and overlaps no operand otherwise.  d <= 16384,
- * d % 4 == 0 (e4m3: d % 16 == 0).  row_mask (nullable): rows with 0 get a
+ * type, and overlaps no operand otherwise.  d <= 16384, d % 4 == 0 (e4m3:
+ * d % 16 == 0); every matrix starts on a boundary of four of its elements
+ * (e4m3: 16 bytes), w on 16 bytes.  row_mask (nullable): rows with 0 get a
  * zero output row; m_tiles (nullable) as in tjb_row_tiles.
  * The 8-bit-capable RMS sibling of fused_add_layernorm
  * (tjkernels/kernels/__init__.py:48-70); no counterpart in the reference.
@@ -437,17 +438,21 @@ int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out, void* out
  * A [M, K] e4m3 (rows lda bytes apart) with scales sa[m, kb] at
  * a_scales[m * a_scales_row + kb * a_scales_blk]; W [N, K] e4m3 (rows ldw
  * bytes apart) with w_scales contiguous [ceil(N/128), ceil(K/128)]; bias fp32
- * [N] or NULL; act: 0 = none, 1 = erf GELU, to 12 x 2^-24 of itself for sums
- * up to 1 in magnitude and to 5e-7 beyond with C in f32, to 5e-7 with the
- * other types (before C's rounding); NaN at minus infinity, as
- * 0.5 x (1 + erf(x / sqrt 2)), and for TJB_E4M3 at plus infinity too.  C (rows
- * ldc elements apart): f32, f16, bf16, or TJB_E4M3 with c_scales contiguous
+ * [N] or NULL; act: 0 = none, 1 = erf GELU (below).  C (rows ldc elements
+ * apart): f32, f16, bf16, or TJB_E4M3 with c_scales contiguous
  * [M, ceil(N/128)].  fp32 accumulation; sa * sw is one fp32 product, so
  * scales whose product leaves the type's normal range lose what it cannot
  * hold.  A call's result depends on nothing but its operands (no atomics, no
- * workspace).  K % 16 == 0, N % 8 == 0 (e4m3 output: N % 16 == 0), both at
- * most 2^31 - 1025; lda, ldw and ldc multiples of 16 bytes; 16-byte aligned A,
- * W, C and bias; C and c_scales overlap no operand.  m_tiles (nullable) as in
+ * workspace); the order in which a row's blocks, parts and bias are added
+ * follows the sizes of the call, so a row's last bits can differ between
+ * batches of different M.
+ * GELU, before C's rounding: for sums up to 1 in magnitude within 12 x 2^-24 of
+ * itself with C in f32 and 3e-6 with the other types, beyond that within 3e-7
+ * and the rounding of fp32.  NaN at minus infinity, as 0.5 x (1 + erf(x / sqrt
+ * 2)), and with TJB_E4M3, where the whole block is lost, at plus infinity too.
+ * K % 16 == 0, N % 8 == 0 (e4m3 output: N % 16 == 0), both at most
+ * 2^31 - 1025; lda, ldw and ldc multiples of 16 bytes; 16-byte aligned A, W, C
+ * and bias; C and c_scales overlap no operand.  m_tiles (nullable) as in
  * tjb_row_tiles.
  * The 8-bit sibling of tjb_gemm_bias; no counterpart in the reference.
  */

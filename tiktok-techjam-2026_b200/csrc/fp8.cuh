@@ -52,7 +52,7 @@ __device__ __forceinline__ float warp_max_abs(float v) {
 // its remainder (Markstein, IBM J. Res. Dev. 34, 1990).  The plain product
 // v * inv moves about one value in 10^6 across a rounding border of the 8-bit
 // type, and full divisions bound the memory-bound kernels here by their
-// instructions (a 65536 x 4096 norm: 540 us against 461).
+// instructions (a 65536 x 4096 norm in its first form: 540 us, 461 with this).
 __device__ __forceinline__ float div_by(float v, float s, float inv) {
   const float q = v * inv;
   return fmaf(fmaf(-q, s, v), inv, q);

@@ -12,11 +12,11 @@
 // operand (TMEM lane = output column n) and the tokens its N operand, so a few
 // tokens cost a narrow MMA and not a padded one.  A call of this size is bound
 // by its chain launch -> first loads -> MMA -> meeting, then by reading the
-// weights (M16 N4096 K4096: 7.2 us, floor 2.6; M48 N16384 K4096 with GELU and
-// an 8-bit output: 18 us, floor 10.4).  The k-blocks of a tile are divided
-// over the CTAs of a cluster (so that enough SMs stream the weights), whose
-// fp32 sums meet in distributed shared memory: CTA r finishes the tokens
-// t = r mod c, adding the CTAs' parts in a fixed order.
+// weights (M16 N4096 K4096: 6.7 us, 2.6 by its bytes; M48 N16384 K4096 with
+// GELU and an 8-bit output: 17.5 us, 10.4 by its bytes).  The k-blocks of a
+// tile are divided over the CTAs of a cluster (so that enough SMs stream the
+// weights), whose fp32 sums meet in distributed shared memory: CTA r finishes
+// the tokens t = r mod c, adding the CTAs' parts in a fixed order.
 //   warp 0      TMA producer: 128 x 128-byte weight and BT x 128-byte token
 //               tiles (128-byte swizzle; one k-block) into a stage ring
 //   warp 1      owns tensor memory, issues the MMAs
@@ -464,7 +464,7 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
   const int64_t tiles = t_tiles * ((args.N + kF8Lanes - 1) / kF8Lanes);
   // As many CTAs per tile as the SMs have room for, at most one per k-block;
   // more than four lose more in their meeting than they gain (M16 N4096 K4096:
-  // 7.2 us with four, 8.0 with eight).
+  // 6.7 us with four, 7.7 with eight).
   const int64_t slots = static_cast<int64_t>(num_sms()) * 2;
   const int kb_count = (args.K + kF8BK - 1) / kF8BK;
   args.splits = 1;
@@ -515,7 +515,8 @@ int launch_skinny(const void* A, const void* W, GemmF8Args args, int lda, int ld
 // hand-over 470, single CTAs 501, those with a loop that is not unrolled 515;
 // accumulators of 128 columns, for more slack, 487: their MMAs are bound by
 // shared memory).  The scaling threads need the registers that warps 0-3 give
-// up (128 x 72 + 256 x 216 = 384 x 168 at launch).  Under a load that lasts,
+// up (128 x 72 + 256 x 216 = 384 x 168 at launch; kSplitK still spills 24 bytes
+// a thread, the other two none).  Under a load that lasts,
 // the board's power limit holds the clock near 1.4 GHz.
 enum WideForm { kWhole, kSplitK, kPaired };
 
@@ -1209,9 +1210,12 @@ extern "C" int tjb_gemm_fp8(const void* A, const float* a_scales, int64_t a_scal
   // More: 64-token tiles (quick to start, their parts quick to meet, but the
   // tensor core a third as busy) or wide ones (pairs, single CTAs, or split over
   // clusters), or wide ones and the rest, by the time that each is expected to
-  // take.  The constants, in us, were fitted to shapes of M 65-16384, N 128-8192,
-  // K 128-16384 on a B200 (mean error 7-9 %); the choice comes within 1 % of the
-  // best of the forms on average, 28 % at worst.
+  // take.  The constants, in us, were fitted on a B200 to shapes of M 65-16384,
+  // N 128-8192, K 128-16384 with fp16 outputs and no activation (mean error 10 %
+  // over 40 other shapes; the choice came within 1 % of the best of the forms on
+  // average, 28 % at worst).  They know neither the output's type nor the
+  // activation: against them 8-bit outputs are 11 % off on average, with GELU 19 %
+  // (always slower), fp32 outputs 15 % and 31 %.
   WideLimits lim;
   if (const int st = wide_limits(lim)) return st;
   const int sms = lim.clusters[0];

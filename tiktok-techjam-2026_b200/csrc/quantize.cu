@@ -13,7 +13,8 @@ constexpr int kQuantThreads = 256;
 // once; 32 (fp32) or 16 (16-bit) neighbouring lanes hold one block, so its
 // amax is a few shuffles of values in registers.  Consecutive warps take
 // consecutive columns.
-// HBM-bound: 16384 x 4096 fp32 52 us, fp16 33 us (floors 51 and 31).
+// HBM-bound: 16384 x 4096 fp32 52 us, fp16 33 us (51 and 31 at the
+// rate of a copy).
 template <typename T, int kSteps>
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(kQuantThreads)
 // three-stage shared-memory ring are in flight (a thread reads only what it
 // copied itself, so the ring needs no barrier).  A CTA per block without the
 // ring left HBM idle while its blocks computed: 16384 x 4096 fp32 78 us, bf16
-// 65 us; with it 57 and 34 (floors 51 and 31).
+// 65 us; with it 57 and 33 (51 and 31 at the rate of a copy).
 constexpr int kRingStages = 3;
 
 template <typename T>

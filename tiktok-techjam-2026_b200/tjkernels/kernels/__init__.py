@@ -664,8 +664,10 @@ def gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales:
              m_tiles: Optional[torch.Tensor] = None):
     """``act(A @ W.T + bias)`` of block-scaled e4m3 operands: ``a`` [M, K] with
     ``a_scales`` [M, ceil(K/128)] (any strides), ``w`` [N, K] with
-    ``w_scales`` [ceil(N/128), ceil(K/128)]; bias fp32 [N].  Each 128-column
-    block's product is scaled and summed in fp32.  ``out_dtype`` fp32, fp16,
+    ``w_scales`` [ceil(N/128), ceil(K/128)]; bias fp32 [N], on a 16-byte
+    boundary.  Each 128-column block's product is scaled and summed in fp32, in
+    an order that follows M, N and K: a row's last bits can differ between
+    batches of different size.  ``out_dtype`` fp32, fp16,
     bf16, or float8_e4m3fn, which returns ``(q, scales)`` as
     :func:`quantize_blocks` of the fp32 result would.  K must be a multiple of
     16, N of 8 (e4m3 output: 16).  ``out``: a [M, N] tensor of ``out_dtype`` to
