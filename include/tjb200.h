@@ -447,7 +447,7 @@ int tjb_add_rmsnorm(const void* res, const void* delta, void* res_out, void* out
  * follows the sizes of the call, so a row's last bits can differ between
  * batches of different M.
  * GELU, before C's rounding: for sums up to 1 in magnitude within 12 x 2^-24 of
- * itself with C in f32 and 3e-6 with the other types, beyond that within 3e-7
+ * itself with C in f32 and 3e-6 with the other types, beyond that within 4e-7
  * and the rounding of fp32.  NaN at minus infinity, as 0.5 x (1 + erf(x / sqrt
  * 2)), and with TJB_E4M3, where the whole block is lost, at plus infinity too.
  * K % 16 == 0, N % 8 == 0 (e4m3 output: N % 16 == 0), both at most

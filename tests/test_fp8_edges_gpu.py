@@ -157,6 +157,20 @@ def test_gelu_blocks_of_the_tail(m):
 
 
 @pytest.mark.parametrize("m", GELU_ROWS)
+def test_gelu_of_large_sums(m):
+    """Up to the largest numbers: themselves, or zero."""
+    x = torch.exp(torch.linspace(math.log(14.0), 88.7, 256, device=DEV))
+    x[-1] = torch.finfo(torch.float32).max
+    x = torch.cat([x, -x])
+    ref = x.clamp_min(0).double().expand(m, -1)
+    for dtype in (torch.float32, torch.bfloat16):
+        out = gelu_of(x, m, dtype)
+        assert torch.equal(out, ref.to(torch.float32).to(dtype))
+    q, s = gelu_of(x, m, F8)
+    check_quantised(q, s, ref.contiguous(), 0.0)
+
+
+@pytest.mark.parametrize("m", GELU_ROWS)
 def test_gelu_of_infinities(m):
     """As 0.5 x (1 + erf(x / sqrt 2)): NaN at minus infinity, infinity at infinity."""
     x = rand(gen(m, 34), 512)

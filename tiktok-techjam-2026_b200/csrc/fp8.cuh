@@ -140,8 +140,8 @@ __device__ __forceinline__ float relu_nan(float x) {
 // 32-bit results, degree 13: Phi(b) to 3e-8 of itself down to -2, 2e-5 to -5
 // and 3e-4 to the end, before the roundings in fp32 (2e-7, 3e-6 and up to 2e-3)
 // and of 2^q (2^-22): for |x| <= 1 the GELU is within 12 x 2^-24 of itself.
-// 16 and 8 bits (a rounding of 2e-4 or more), degree 7: the GELU to 3e-7
-// absolute, 3e-6 of itself for |x| <= 2, 8e-4 to -5.5, 0.012 to -9 and a tenth
+// 16 and 8 bits (a rounding of 2e-4 or more), degree 7: the GELU to 4e-7
+// absolute, 4e-6 of itself for |x| <= 2, 8e-4 to -5.5, 0.012 to -9 and a tenth
 // to the end.
 // Infinities: the factor of a negative x is not cut, and minus infinity times
 // zero is NaN, as in 0.5 x (1 + erf(x / sqrt 2)); plus infinity stays.  For 8
